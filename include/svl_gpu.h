@@ -85,7 +85,8 @@ typedef struct svl_text_config {
   const svl_layer_config* layers; /* num_hidden_layers entries */
 } svl_text_config;
 
-typedef enum svl_dtype { SVL_DTYPE_F32 = 0, SVL_DTYPE_BF16 = 1 } svl_dtype;
+/* SVL_DTYPE_F16 is an operand type of the operators below; weight tensors are F32 or BF16. */
+typedef enum svl_dtype { SVL_DTYPE_F32 = 0, SVL_DTYPE_BF16 = 1, SVL_DTYPE_F16 = 2 } svl_dtype;
 
 /* One named weight tensor in host memory (a Safetensors entry,
  * src/binary/safetensors.rs:69-123).  BF16 data is widened to FP32 exactly
@@ -353,6 +354,177 @@ int svl_search_noalloc(const float* d_rows, const uint64_t* d_chunk_ids, uint64_
                        const float* d_queries, uint32_t n_queries, const uint8_t* d_row_mask, uint32_t k,
                        uint64_t* d_out_rows, uint64_t* d_out_chunk_ids, double* d_out_scores,
                        uint32_t* d_out_counts, void* stream, char* err, size_t err_len);
+
+/* ------------------------------------------------------------- operators --
+ * Blocks of the towers and encoders that stand beside the text model: what
+ * makes the soft tokens of svl_feature_span, or another encoder's rows, from
+ * projections (svl_q4_linear_device), positions (svl_rope_apply_device) and
+ * attention (svl_attention_device).  The reference runs these towers on the
+ * CPU; the entry points have no one counterpart there.
+ *
+ * Operands are rows of device memory: row t starts at pointer + t * ld
+ * elements and holds its heads one after another, as the fused q, k, v rows
+ * of a projection do.  Every pointer belongs to the device of the handle (or
+ * of the `device` argument), whatever the calling thread's current device is,
+ * which stays as it was.  The *_device calls and the frees of the handles
+ * follow `stream` (NULL = the legacy default stream): they return once
+ * queued, allocate nothing and never wait, so they may be captured into a
+ * CUDA graph; a captured call keeps referring to the handle, which has to
+ * outlive the graph.  A handle is never changed by a call, so threads,
+ * streams and graphs may share it; outputs and workspaces are the caller's
+ * and must not be shared by calls that may overlap.  Outputs must not overlap
+ * inputs except where stated.  NULL pointers are accepted where nothing is
+ * read or written through them. */
+
+/* How the axes of a multi-axis rotary embedding share a head.  An axis with n
+ * pairs turns n pairs of dimensions by angles position * frequency:
+ *   SVL_ROPE_SPLIT        axis a owns the next 2 n_a dimensions and pairs d
+ *                         with d + n_a inside them; pair i has the frequency
+ *                         theta[a]^(-i / n_a).  (Images: half a head turns
+ *                         with the row, half with the column.)
+ *   SVL_ROPE_SECTIONS     with n = sum n_a, pair p is (p, p + n) and has the
+ *                         frequency theta[0]^(-p / n); each axis owns a run of
+ *                         pairs, in order.
+ *   SVL_ROPE_INTERLEAVED  the same pairs and frequencies, dealt to the axes
+ *                         in turn, an axis dropping out once it has its n_a.
+ * Dimensions behind 2 * sum n_a are copied. */
+typedef enum svl_rope_arrangement {
+  SVL_ROPE_SPLIT = 0,
+  SVL_ROPE_SECTIONS = 1,
+  SVL_ROPE_INTERLEAVED = 2
+} svl_rope_arrangement;
+
+#define SVL_ROPE_MAX_AXES 4u
+#define SVL_ROPE_MAX_HEAD_DIM 512u
+
+typedef struct svl_rope_config {
+  uint32_t head_dim;             /* 2..SVL_ROPE_MAX_HEAD_DIM */
+  uint32_t n_axes;               /* 1..SVL_ROPE_MAX_AXES */
+  uint32_t pairs[4];             /* per axis; >= 1 for the first n_axes, 2 * sum <= head_dim */
+  uint32_t arrangement;          /* svl_rope_arrangement */
+  uint32_t reserved;             /* zero */
+  double theta[4];               /* finite, > 0; theta[0] alone unless SVL_ROPE_SPLIT */
+} svl_rope_config;
+
+typedef struct svl_rope svl_rope;
+
+/* A rotary embedding's tables, in host memory: no device is touched, and any
+ * device may use it.  A bad configuration -> SVL_USAGE. */
+int svl_rope_create(const svl_rope_config* config, svl_rope** out, char* err, size_t err_len);
+void svl_rope_destroy(svl_rope* rope);
+
+/* Rotates n_tokens rows of q_heads query heads and k_heads key heads (either
+ * may be 0) of `dtype` (svl_dtype).  d_positions: n_axes x n_tokens, one axis
+ * after another, any int32 values; angles are exact to 2^-32 of a turn however
+ * far the position, and products are rounded once to the type.  An output may
+ * be its own input (same pointer and ld: in place).  Element alignment
+ * suffices; 16-byte aligned rows with an even head are faster.  ld >= heads *
+ * head_dim, n_tokens < 2^31 (else SVL_USAGE). */
+int svl_rope_apply_device(const svl_rope* rope, int device, uint32_t dtype, const int32_t* d_positions,
+                          uint64_t n_tokens, const void* d_q, uint64_t ld_q, uint32_t q_heads, void* d_q_out,
+                          uint64_t ld_q_out, const void* d_k, uint64_t ld_k, uint32_t k_heads, void* d_k_out,
+                          uint64_t ld_k_out, void* stream, char* err, size_t err_len);
+
+/* Attention over packed sequences: for query i of a sequence (of n_q queries
+ * and n_k keys) at position p = i + n_k - n_q, and key j,
+ *   visible(i, j) = doc_q[i] == doc_k[j], or j < prefix        (documents)
+ *                   and doc_q[i] >= 0 and doc_k[j] >= 0
+ *                   and (j < prefix, or j <= p if causal)      (order)
+ *                   and (j < prefix, or |p - j| <= window if window >= 0)
+ *   t(i, j) = scale * q_i . k_j;  cap > 0: t = cap * tanh(t / cap)
+ *             then t -= slope[head] * |p - j|
+ *   out_i   = sum over the visible j of softmax(t)_j v_j
+ *   lse_i   = log of the sum over the visible j of exp(t(i, j))
+ * A row that sees no key gets out = 0 and lse = -inf.  A masked key's values
+ * never reach a row, be they NaN or infinite; rows of other sequences and
+ * rows behind the last one are neither read into a result nor written.
+ * Scores, softmax statistics and sums are FP32 (FP16 / BF16: the weights of
+ * the visible keys are rounded to the type before they multiply v). */
+typedef struct svl_attention_config {
+  uint32_t dtype;                /* svl_dtype of q, k, v and out */
+  uint32_t q_heads;              /* a multiple of kv_heads; q_heads / kv_heads <= 65535 */
+  uint32_t kv_heads;             /* 1..65535; query head h reads kv head h / (q_heads / kv_heads) */
+  uint32_t head_dim;             /* 1..512 */
+  float scale;                   /* finite, > 0 */
+  float cap;                     /* 0 = none; finite, > 0 */
+  uint32_t causal;               /* 0 or 1 */
+  int32_t window;                /* < 0 = none */
+  uint32_t reserved[4];          /* zero */
+} svl_attention_config;
+
+typedef struct svl_attention_plan svl_attention_plan;
+
+/* Checks a batch's layout and masks and puts its tile schedule on `device`.
+ * Host pointers, copied; synchronous.  One plan serves every layer that
+ * attends over the batch.
+ *   cu_q, cu_k : batch + 1 offsets each, as cu_seqlens; cu_k NULL = cu_q
+ *   prefix     : batch entries, or NULL (0 for all)
+ *   doc_q, doc_k : the document of every packed query / key, or both NULL;
+ *                any values, negative = padding; doc_k NULL alone = doc_q, if
+ *                cu_k is NULL too
+ *   slopes     : q_heads finite values, or NULL
+ * Errors: SVL_USAGE (bad configuration, offsets that start off 0 or fall,
+ * non-finite slopes), SVL_LIMIT_EXCEEDED (2^31 or more keys, or query rows
+ * times group, in one sequence; out of memory). */
+int svl_attention_plan_create(int device, const svl_attention_config* config, const uint64_t* cu_q,
+                              const uint64_t* cu_k, uint32_t batch, const uint64_t* prefix, const int32_t* doc_q,
+                              const int32_t* doc_k, const float* slopes, svl_attention_plan** out, char* err,
+                              size_t err_len);
+void svl_attention_plan_destroy(svl_attention_plan* plan);
+
+/* Bytes of workspace that svl_attention_device needs (0 unless the plan cuts
+ * a long key axis over several blocks). */
+int svl_attention_plan_workspace(const svl_attention_plan* plan, uint64_t* bytes);
+
+/* One attention over the plan's batch.  d_lse: q rows x q_heads, or NULL.
+ * d_workspace: 16-byte aligned, svl_attention_plan_workspace bytes, contents
+ * irrelevant before and after.  ld >= heads * head_dim.  With FP16 / BF16 and
+ * a head_dim that is a multiple of 8, q, k, v and out have to be 16-byte
+ * aligned with ld a multiple of 8 (else SVL_USAGE); otherwise element
+ * alignment suffices. */
+int svl_attention_device(const svl_attention_plan* plan, const void* d_q, uint64_t ld_q, const void* d_k,
+                         uint64_t ld_k, const void* d_v, uint64_t ld_v, void* d_out, uint64_t ld_out, float* d_lse,
+                         void* d_workspace, uint64_t workspace_bytes, void* stream, char* err, size_t err_len);
+
+/* Synchronises the plan's device and reports a deferred device-side error (a
+ * bounded wait that ran out -> SVL_INTERNAL). */
+int svl_attention_check(const svl_attention_plan* plan, char* err, size_t err_len);
+
+/* A weight matrix W [n, k] in 4 bits: W[i, j] = (code - zero) * scale with
+ * codes and zeros 0..15 and one scale (and zero) per row and group of `group`
+ * columns (32, 64 or 128; k a multiple of it, n and k below 2^31). */
+typedef struct svl_q4 svl_q4;
+
+/* From existing codes, in host or in device memory (work that writes them has
+ * to be complete); copied into the handle's own layout; synchronous.
+ *   codes  : n x k/2 bytes, column 2c in the low half of byte c
+ *   scales : n x k/group of scale_dtype (SVL_DTYPE_F16 or SVL_DTYPE_BF16)
+ *   zeros  : n x k/group bytes (the low four bits), or NULL (8 for all) */
+int svl_q4_create(int device, const uint8_t* codes, const void* scales, uint32_t scale_dtype, const uint8_t* zeros,
+                  uint32_t n, uint32_t k, uint32_t group, svl_q4** out, char* err, size_t err_len);
+
+/* Quantises a host weight tensor (2-D, F32 or BF16) on the device: per group,
+ * with asymmetric = 0 scale = max|w| / 7 and zero 8 (codes 1..15), else scale
+ * = (max - min) / 15 over the values and 0, and zero = -min / scale rounded;
+ * scales are rounded to BF16 before the codes are chosen, codes are the
+ * nearest (ties to even).  A non-finite weight -> SVL_CORRUPT. */
+int svl_q4_quantize(int device, const svl_tensor_view* weight, uint32_t group, uint32_t asymmetric, svl_q4** out,
+                    char* err, size_t err_len);
+void svl_q4_destroy(svl_q4* weight);
+
+/* The matrix as svl_q4_create takes it, into host memory (any pointer may be
+ * NULL): sizes and scale type, codes, scales, zeros (all 8 when it has none). */
+int svl_q4_read(const svl_q4* weight, uint32_t* n, uint32_t* k, uint32_t* group, uint32_t* scale_dtype,
+                uint8_t* codes, void* scales, uint8_t* zeros, char* err, size_t err_len);
+
+/* y = x W^T: `rows` rows of x (k values each, row stride ld_x) into y (n
+ * values, row stride ld_y), both of `dtype`.  Made for few rows (a query's
+ * tokens, down to a single one); any count below 2^31 works.  Products and
+ * sums are FP32 (an F32 x keeps its 24 bits), y is rounded once.  A row with a
+ * NaN or infinite value gets non-finite results; the others do not.  Element
+ * alignment suffices.  Columns of y behind n are left as they were. */
+int svl_q4_linear_device(const svl_q4* weight, uint32_t dtype, const void* d_x, uint64_t ld_x, uint64_t rows,
+                         void* d_y, uint64_t ld_y, void* stream, char* err, size_t err_len);
 
 #ifdef __cplusplus
 }

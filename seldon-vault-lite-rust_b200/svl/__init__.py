@@ -11,6 +11,9 @@ libsvl_gpu.so (include/svl_gpu.h):
 * svl.bundle.Bundle / load_text_model  -- src/bundle/mod.rs, src/model/source.rs (include/svl_bundle.h)
 * svl.index.VectorIndex / rank / Index -- src/index/vector.rs, src/index/mod.rs
 * svl.config.TextConfig                -- src/model/config.rs
+* svl.ops                              -- operators of the towers beside the text model:
+                                          multi-axis rotary positions, masked attention,
+                                          4-bit linears (device buffers)
 * svl.errors                           -- src/error.rs
 * svl.dist                             -- data-parallel encoder and row-sharded
                                           search over one process per GPU

@@ -73,8 +73,34 @@ class SvlFeatureSpan(ctypes.Structure):
     ]
 
 
+class SvlRopeConfig(ctypes.Structure):
+    _fields_ = [
+        ("head_dim", c_u32),
+        ("n_axes", c_u32),
+        ("pairs", c_u32 * 4),
+        ("arrangement", c_u32),
+        ("reserved", c_u32),
+        ("theta", ctypes.c_double * 4),
+    ]
+
+
+class SvlAttentionConfig(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_u32),
+        ("q_heads", c_u32),
+        ("kv_heads", c_u32),
+        ("head_dim", c_u32),
+        ("scale", c_f32),
+        ("cap", c_f32),
+        ("causal", c_u32),
+        ("window", ctypes.c_int32),
+        ("reserved", c_u32 * 4),
+    ]
+
+
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_F16 = 2
 
 # name -> (restype, argtypes); every int-returning call returns svl_status
 PROTOTYPES = {
@@ -106,6 +132,19 @@ PROTOTYPES = {
     "svl_allgather_rows": (ctypes.c_int, [c_ptr, c_ptr, c_u64, c_u32, c_ptr, c_ptr, c_char_p, c_size]),
     "svl_sharded_search": (ctypes.c_int, [c_ptr, c_ptr, c_u64, c_ptr, c_u32, c_u32, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_char_p, c_size]),
     "svl_search_noalloc": (ctypes.c_int, [c_ptr, c_ptr, c_u64, c_u32, c_ptr, c_u32, c_ptr, c_u32, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_char_p, c_size]),
+    "svl_rope_create": (ctypes.c_int, [ctypes.POINTER(SvlRopeConfig), ctypes.POINTER(c_ptr), c_char_p, c_size]),
+    "svl_rope_destroy": (None, [c_ptr]),
+    "svl_rope_apply_device": (ctypes.c_int, [c_ptr, ctypes.c_int, c_u32, c_ptr, c_u64, c_ptr, c_u64, c_u32, c_ptr, c_u64, c_ptr, c_u64, c_u32, c_ptr, c_u64, c_ptr, c_char_p, c_size]),
+    "svl_attention_plan_create": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(SvlAttentionConfig), c_ptr, c_ptr, c_u32, c_ptr, c_ptr, c_ptr, c_ptr, ctypes.POINTER(c_ptr), c_char_p, c_size]),
+    "svl_attention_plan_destroy": (None, [c_ptr]),
+    "svl_attention_plan_workspace": (ctypes.c_int, [c_ptr, ctypes.POINTER(c_u64)]),
+    "svl_attention_device": (ctypes.c_int, [c_ptr, c_ptr, c_u64, c_ptr, c_u64, c_ptr, c_u64, c_ptr, c_u64, c_ptr, c_ptr, c_u64, c_ptr, c_char_p, c_size]),
+    "svl_attention_check": (ctypes.c_int, [c_ptr, c_char_p, c_size]),
+    "svl_q4_create": (ctypes.c_int, [ctypes.c_int, c_ptr, c_ptr, c_u32, c_ptr, c_u32, c_u32, c_u32, ctypes.POINTER(c_ptr), c_char_p, c_size]),
+    "svl_q4_quantize": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(SvlTensorView), c_u32, c_u32, ctypes.POINTER(c_ptr), c_char_p, c_size]),
+    "svl_q4_destroy": (None, [c_ptr]),
+    "svl_q4_read": (ctypes.c_int, [c_ptr, ctypes.POINTER(c_u32), ctypes.POINTER(c_u32), ctypes.POINTER(c_u32), ctypes.POINTER(c_u32), c_ptr, c_ptr, c_ptr, c_char_p, c_size]),
+    "svl_q4_linear_device": (ctypes.c_int, [c_ptr, c_u32, c_ptr, c_u64, c_u64, c_ptr, c_u64, c_ptr, c_char_p, c_size]),
 }
 
 PACKAGE_ROOT = Path(__file__).resolve().parent.parent
