@@ -87,4 +87,12 @@ SVL_DEV bool sees(const AttnParams& p, const RowMask& m, uint32_t j, int32_t doc
   return j < m.n_k && m.doc >= 0 && doc >= 0 && (ahead || (near && doc == m.doc));
 }
 
+// The tcgen05 kernel for FP16 and BF16 (ops_attention_tc.cu).
+bool attention_tc_takes(const svl_attention_config& c, uint64_t total_q, uint64_t total_k);
+// Rows of a row tile (whole queries: a multiple of the group) and row tiles of
+// a segment.
+uint32_t attention_tc_tile_rows(uint32_t group);
+uint32_t attention_tc_row_tiles(uint32_t head_dim);
+cudaError_t attention_tc_launch(const AttnParams& p, uint32_t dtype, cudaStream_t st);
+
 }  // namespace svl
