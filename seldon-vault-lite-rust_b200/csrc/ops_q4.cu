@@ -13,6 +13,7 @@
 // is exact, and the parts are further columns of the product.
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
 #include <vector>
 
 #include "ops_common.cuh"
@@ -22,10 +23,6 @@ namespace {
 
 constexpr uint32_t kErrNonFinite = 1;
 
-SVL_DEV float scale_of(uint16_t bits, uint32_t dtype) {
-  return dtype == SVL_DTYPE_F16 ? __half2float(__ushort_as_half(bits)) : __uint_as_float((uint32_t)bits << 16);
-}
-
 // The order of the product's columns inside a block of 64 is free as long as
 // both operands have it.  Lane 4 g + q takes columns 8 q .. 8 q + 7 of each half
 // block of 32 (the shortest group), four of them a step: steps 0 and 1 are the
@@ -33,31 +30,34 @@ SVL_DEV float scale_of(uint16_t bits, uint32_t dtype) {
 // loads and its codes of the block's 16 x 64 weights one: word w holds step w,
 // for rows g and g + 8.  The two nibbles of an operand register lie 16 bits
 // apart, where one mask takes both.
+//
+// A row block (16 weight rows) is a run of spans of 128 columns: two blocks'
+// codes, and in arrays of their own the span's 128 / group scale pairs and
+// zeros.  Rows and columns behind the matrix have code 0 and scale 0.
 struct Q4Matrix {
-  const uint4* codes;      // [row block of 16][column block of 64][lane]
-  const uint32_t* scales;  // [row block][group][8]: rows g (low half) and g + 8
-  const uint16_t* zeros;   // the same, a byte each; NULL: 8
+  const uint4* codes;      // [row block][span][block][lane]
+  const uint32_t* scales;  // [row block][span][group][8]: rows g (low half) and g + 8
+  const uint8_t* zeros;    // the same, four bits each; NULL: 8
   uint32_t n, k, group, scale_dtype;
   __host__ __device__ uint32_t row_blocks() const { return (n + 15) / 16; }
-  __host__ __device__ uint32_t col_blocks() const { return (k + 63) / 64; }
-  __host__ __device__ uint32_t groups() const { return k / group; }
+  __host__ __device__ uint32_t spans() const { return (k + 127) / 128; }
+  __host__ __device__ uint32_t span_groups() const { return 128 / group; }
 };
 
 // Nibble of a word that holds row g + 8 upper and the step's column c = 0..3:
 // register upper + 2 (c / 2) of the operand, half c % 2.
 SVL_DEV uint32_t nibble_at(uint32_t upper, uint32_t c) { return upper + 2 * (c >> 1) + 4 * (c & 1); }
 
-// Plain codes, scales and zeros into the handle's order; rows and columns
-// behind the matrix get code 0 and scale 0.
+// Plain codes, scales and zeros into the handle's order.
 __global__ void q4_lay_out_kernel(const __grid_constant__ Q4Matrix m, const uint8_t* __restrict__ codes,
                                   const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros) {
-  const uint64_t words = (uint64_t)m.row_blocks() * m.col_blocks() * 128, step = (uint64_t)gridDim.x * blockDim.x;
+  const uint64_t words = (uint64_t)m.row_blocks() * m.spans() * 256, step = (uint64_t)gridDim.x * blockDim.x;
   const uint64_t first = blockIdx.x * (uint64_t)blockDim.x + threadIdx.x;
   for (uint64_t i = first; i < words; i += step) {
-    const uint32_t w = i & 3, lane = (i >> 2) & 31;
-    const uint64_t block = i >> 7;
-    const uint64_t row = block / m.col_blocks() * 16 + (lane >> 2);
-    const uint64_t col = block % m.col_blocks() * 64 + (w >> 1) * 32 + (lane & 3) * 8 + 4 * (w & 1);
+    const uint32_t w = i & 3, lane = (i >> 2) & 31, half = (i >> 7) & 1;
+    const uint64_t span = i >> 8;
+    const uint64_t row = span / m.spans() * 16 + (lane >> 2);
+    const uint64_t col = span % m.spans() * 128 + half * 64 + (w >> 1) * 32 + (lane & 3) * 8 + 4 * (w & 1);
     uint32_t word = 0;
     for (uint32_t upper = 0; upper < 2; ++upper)
       if (row + 8 * upper < m.n && col < m.k) {
@@ -67,18 +67,18 @@ __global__ void q4_lay_out_kernel(const __grid_constant__ Q4Matrix m, const uint
       }
     ((uint32_t*)m.codes)[i] = word;
   }
-  const uint64_t pairs = (uint64_t)m.row_blocks() * m.groups() * 8;
-  for (uint64_t i = first; i < pairs; i += step) {
-    const uint64_t row = i / 8 / m.groups() * 16 + (i & 7), g = i / 8 % m.groups();
+  const uint32_t per_row = m.spans() * m.span_groups(), groups = m.k / m.group;
+  for (uint64_t i = first; i < (uint64_t)m.row_blocks() * per_row * 8; i += step) {
+    const uint64_t row = i / 8 / per_row * 16 + (i & 7), g = i / 8 % per_row;
     uint32_t s = 0, z = 0;
     for (uint32_t upper = 0; upper < 2; ++upper)
-      if (row + 8 * upper < m.n) {
-        const uint64_t at = (row + 8 * upper) * m.groups() + g;
+      if (row + 8 * upper < m.n && g < groups) {
+        const uint64_t at = (row + 8 * upper) * groups + g;
         s |= (uint32_t)scales[at] << (16 * upper);
-        if (zeros) z |= (uint32_t)(zeros[at] & 15) << (8 * upper);
+        if (zeros) z |= (uint32_t)(zeros[at] & 15) << (4 * upper);
       }
     ((uint32_t*)m.scales)[i] = s;
-    if (zeros) ((uint16_t*)m.zeros)[i] = (uint16_t)z;
+    if (zeros) ((uint8_t*)m.zeros)[i] = (uint8_t)z;
   }
 }
 
@@ -88,16 +88,17 @@ __global__ void q4_read_kernel(const __grid_constant__ Q4Matrix m, uint8_t* __re
   const uint64_t step = (uint64_t)gridDim.x * blockDim.x, first = blockIdx.x * (uint64_t)blockDim.x + threadIdx.x;
   for (uint64_t i = first; codes && i < (uint64_t)m.n * (m.k / 2); i += step) {
     const uint64_t row = i / (m.k / 2), col = i % (m.k / 2) * 2;
-    const uint64_t block = row / 16 * m.col_blocks() + col / 64;
+    const uint64_t block = (row / 16 * m.spans() + col / 128) * 2 + (col & 127) / 64;
     const uint32_t lane = (row & 7) * 4 + (col & 31) / 8, w = (col & 63) / 32 * 2 + (col & 7) / 4, upper = row >> 3 & 1;
     const uint32_t word = ((const uint32_t*)m.codes)[block * 128 + lane * 4 + w];
     codes[i] = (uint8_t)((word >> (4 * nibble_at(upper, col & 3)) & 15) | (word >> (4 * nibble_at(upper, (col & 3) + 1)) & 15) << 4);
   }
-  for (uint64_t i = first; i < (uint64_t)m.n * m.groups(); i += step) {
-    const uint64_t row = i / m.groups(), at = (row / 16 * m.groups() + i % m.groups()) * 8 + (row & 7);
+  const uint32_t per_row = m.spans() * m.span_groups(), groups = m.k / m.group;
+  for (uint64_t i = first; i < (uint64_t)m.n * groups; i += step) {
+    const uint64_t row = i / groups, at = (row / 16 * per_row + i % groups) * 8 + (row & 7);
     const uint32_t upper = row >> 3 & 1;
     if (scales) scales[i] = (uint16_t)(m.scales[at] >> (16 * upper));
-    if (zeros) zeros[i] = m.zeros ? (uint8_t)(m.zeros[at] >> (8 * upper)) : 8;
+    if (zeros) zeros[i] = m.zeros ? (uint8_t)(m.zeros[at] >> (4 * upper) & 15) : 8;
   }
 }
 
@@ -114,6 +115,20 @@ SVL_DEV void mma_16816(__nv_bfloat16, float* d, const uint32_t* a, const uint32_
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
+// The same with nothing to add to.
+SVL_DEV void mma_16816_first(__half, float* d, const uint32_t* a, const uint32_t* b) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.0f));
+}
+SVL_DEV void mma_16816_first(__nv_bfloat16, float* d, const uint32_t* a, const uint32_t* b) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.0f));
+}
+
 // 16-bit operands of the product; FP32 rows take the BF16 form three times.
 template <typename T>
 struct Operand {
@@ -127,18 +142,18 @@ struct Operand<float> {
 };
 
 // A whole number q of 4 bits in a half: 1024 + q is FP16 0x6400 | q, 128 + q is
-// BF16 0x4300 | q; the zero comes with the same offset and both differences are
-// exact.
+// BF16 0x4300 | q; the zero comes with the same offset, negated (the sign bit),
+// and the sums are exact.
 SVL_DEV uint32_t offset_bits(__half) { return 0x64006400u; }
 SVL_DEV uint32_t offset_bits(__nv_bfloat16) { return 0x43004300u; }
-SVL_DEV uint32_t minus(__half, uint32_t a, uint32_t b) {
+SVL_DEV uint32_t plus(__half, uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-SVL_DEV uint32_t minus(__nv_bfloat16, uint32_t a, uint32_t b) {
+SVL_DEV uint32_t plus(__nv_bfloat16, uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(0x3f803f80u), "r"(b));
   return r;
 }
 
@@ -158,139 +173,383 @@ SVL_DEV uint32_t bf16_part(float x, int part) {
 }
 
 // 8 values of a row of x as two steps' operand registers (two a step).
-template <typename T, bool WIDE>
-SVL_DEV void load_columns(const T* row, int part, uint32_t* b) {
+template <typename T>
+SVL_DEV void pack_columns(const uint4* v, int part, uint32_t* b) {
   if constexpr (sizeof(T) == 2) {
-    if constexpr (WIDE) {
-      const uint4 v = *(const uint4*)row;
-      b[0] = v.x, b[1] = v.y, b[2] = v.z, b[3] = v.w;
-    } else {
-      const uint16_t* v = (const uint16_t*)row;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b[i] = (uint32_t)v[2 * i] | (uint32_t)v[2 * i + 1] << 16;
-    }
+    b[0] = v->x, b[1] = v->y, b[2] = v->z, b[3] = v->w;
   } else {
-    float x[8];
-    if constexpr (WIDE) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float4 v = *(const float4*)((const float*)row + 4 * i);
-        x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = row[i];
+    for (int i = 0; i < 2; ++i) {
+      const float x[4] = {__uint_as_float(v[i].x), __uint_as_float(v[i].y), __uint_as_float(v[i].z), __uint_as_float(v[i].w)};
+      b[2 * i] = bf16_part(x[0], part) >> 16 | bf16_part(x[1], part);
+      b[2 * i + 1] = bf16_part(x[2], part) >> 16 | bf16_part(x[3], part);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = bf16_part(x[2 * i], part) >> 16 | bf16_part(x[2 * i + 1], part);
   }
+}
+// From global memory, with the element's own alignment.
+template <typename T>
+SVL_DEV void load_columns(const T* row, int part, uint32_t* b) {
+  uint4 v[sizeof(T) / 2];
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t* e = (const uint16_t*)row;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)e[2 * i] | (uint32_t)e[2 * i + 1] << 16;
+    v[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    const uint32_t* e = (const uint32_t*)row;
+    v[0] = make_uint4(e[0], e[1], e[2], e[3]);
+    v[1] = make_uint4(e[4], e[5], e[6], e[7]);
+  }
+  pack_columns<T>(v, part, b);
+}
+
+// Asynchronous copies to shared memory.  `there` false: 16 zero bytes, nothing is read.
+SVL_DEV void copy16(uint32_t smem, const void* src, bool there = true) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+SVL_DEV void copy4(uint32_t smem, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem), "l"(src) : "memory");
+}
+SVL_DEV void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+SVL_DEV void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 constexpr int kWarps = 8;
 
-// One block: 16 R weight rows against 8 NT columns (rows of x, or parts of
-// them); its warps take the column blocks in turn and join their sums in shared
-// memory, in a fixed order.  SHORT: groups of 32 (two a block of 64).
-template <typename T, int NT, int R, bool SHORT, bool WIDE>
-__global__ void __launch_bounds__(kWarps * 32)
-    q4_linear_kernel(const __grid_constant__ Q4Matrix w, const T* __restrict__ x, uint64_t ld_x, uint64_t rows,
-                     T* __restrict__ y, uint64_t ld_y) {
-  using Op = typename Operand<T>::Type;
-  constexpr int kParts = Operand<T>::kParts, kCols = NT * 8, kRows = kCols / kParts;
-  constexpr int kDeep = NT == 1 ? 4 : 2;  // column blocks in flight
-  extern __shared__ float sums[];         // [warp][16 R][kCols]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const uint32_t col_blocks = w.col_blocks(), groups = w.groups(), row_blocks = w.row_blocks();
-  const uint32_t rb0 = blockIdx.x * R;
-  const uint64_t m0 = (uint64_t)blockIdx.y * kRows;
-  float acc[R][NT][4] = {};
+// A span's weights in shared memory.
+template <int GROUP>
+struct Weights {
+  static constexpr int kGroups = 128 / GROUP;
+  uint4 code[2][32];
+  uint32_t scale[kGroups][8];
+  uint8_t zero[kGroups][8];
+  uint8_t unused[128 - kGroups * 40 % 128];
+};
+static_assert(sizeof(Weights<32>) % 128 == 0 && sizeof(Weights<64>) % 128 == 0 && sizeof(Weights<128>) % 128 == 0,
+              "whole lines");
 
-  for (uint32_t kb0 = warp; kb0 < col_blocks; kb0 += kWarps * kDeep) {
-    uint4 code[kDeep][R];
-    uint32_t scale[kDeep][R][SHORT ? 2 : 1], zero[kDeep][R][SHORT ? 2 : 1];
+// A lane's part in the copies of one row block's spans, one after another from
+// `first` on.
+template <int GROUP, bool ZEROS>
+struct WeightCopies {
+  using W = Weights<GROUP>;
+  const uint4* code;
+  const uint32_t* scale;
+  const uint8_t* zero;
+  SVL_DEV WeightCopies(const Q4Matrix& w, uint64_t rb, uint32_t first, int lane) {
+    const uint64_t span = rb * w.spans() + first;
+    code = w.codes + span * 64 + lane;
+    scale = w.scales + span * W::kGroups * 8 + lane;
+    if (ZEROS) zero = w.zeros + span * W::kGroups * 8 + lane * 4;
+  }
+  // Span `i` from here into shared memory; `to` includes this lane's 16 bytes.
+  SVL_DEV void copy(uint32_t to, int i, int lane) const {
+    copy16(to, code + i * 64);
+    copy16(to + 512, code + i * 64 + 32);
+    const uint32_t side = to - lane * 12;
+    if (W::kGroups == 4 || lane < W::kGroups * 8) copy4(side + (uint32_t)offsetof(W, scale), scale + i * W::kGroups * 8);
+    if (ZEROS && lane < W::kGroups * 2) copy4(side + (uint32_t)offsetof(W, zero), zero + i * W::kGroups * 8);
+  }
+  SVL_DEV void advance(int spans) {
+    code += spans * 64;
+    scale += spans * W::kGroups * 8;
+    if (ZEROS) zero += spans * W::kGroups * 8;
+  }
+};
+
+template <bool HALF>
+SVL_DEV float2 scale_pair(uint32_t s) {
+  return HALF ? unpack_half2(s) : make_float2(__uint_as_float(s << 16), __uint_as_float(s & 0xffff0000u));
+}
+
+// acc += (codes - zeros) . columns * scales over a span, a group at a time;
+// b[block] are a lane's four steps of operand registers of a column tile.
+// SETS column tiles share the unpacked weights.
+template <typename Op, int GROUP, bool HALF, bool ZEROS, int SETS, typename Columns>
+SVL_DEV void multiply_span(float (*acc)[4], const Weights<GROUP>& st, int lane, Columns&& columns) {
+  const int g = lane >> 2;
+  const uint32_t base = offset_bits(Op());
+  uint32_t a[2][4][4];
 #pragma unroll
-    for (int d = 0; d < kDeep; ++d)
+  for (int half = 0; half < 2; ++half) {
+    const uint4 code = st.code[half][lane];
+    const uint32_t word[4] = {code.x, code.y, code.z, code.w};
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const uint32_t kb = kb0 + d * kWarps, rb = rb0 + r;
-        const bool in = kb < col_blocks && rb < row_blocks;
-        code[d][r] = in ? __ldcs(w.codes + ((uint64_t)rb * col_blocks + kb) * 32 + lane) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int h = 0; h < (SHORT ? 2 : 1); ++h) {
-          const uint32_t gr = SHORT ? 2 * kb + h : kb * 64 / w.group;
-          const bool there = in && gr < groups;
-          const uint64_t at = ((uint64_t)rb * groups + gr) * 8 + g;
-          scale[d][r][h] = there ? __ldcs(w.scales + at) : 0;
-          zero[d][r][h] = w.zeros ? (there ? __ldcs(w.zeros + at) : 0) : 0x0808;
-        }
+    for (int i = 0; i < 4; ++i) {
+      const int group = (half * 64 + i / 2 * 32) / GROUP;
+      uint32_t z0 = (base | 0x80008000u) + 0x00080008u, z1 = z0;
+      if (ZEROS) {
+        const uint32_t z = st.zero[group][g];
+        z0 = (base | 0x80008000u) + (z & 15) * 0x10001u, z1 = (base | 0x80008000u) + (z >> 4) * 0x10001u;
       }
 #pragma unroll
-    for (int d = 0; d < kDeep; ++d) {
-      const uint32_t kb = kb0 + d * kWarps;
-      if (kb >= col_blocks) break;
-      uint32_t a[R][4][4];
+      for (int e = 0; e < 4; ++e) a[half][i][e] = plus(Op(), (word[i] >> (4 * e) & 0x000f000fu) | base, e & 1 ? z1 : z0);
+    }
+  }
+  float2 scale[Weights<GROUP>::kGroups];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const uint32_t word[4] = {code[d][r].x, code[d][r].y, code[d][r].z, code[d][r].w};
-        const uint32_t base = offset_bits(Op());
+  for (int i = 0; i < Weights<GROUP>::kGroups; ++i) scale[i] = scale_pair<HALF>(st.scale[i][g]);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const uint32_t z = zero[d][r][SHORT ? s >> 1 : 0];
-          const uint32_t z0 = base + (z & 15) * 0x10001u, z1 = base + (z >> 8 & 15) * 0x10001u;
+  for (int t = 0; t < SETS; ++t) {
+    uint32_t b[2][8];
+    columns(t, b);
+    // a chain of products for each group, two for the span's only one
+    constexpr int kChain = GROUP == 32 ? 2 : 4;
+    float part[8 / kChain][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            a[r][s][i] = minus(Op(), (word[s] >> (4 * i) & 0x000f000fu) | base, i & 1 ? z1 : z0);
-        }
-      }
-      const uint32_t col = kb * 64 + q * 8;
-      const bool second = kb * 64 + 32 < w.k;  // k is a multiple of 32
+    for (int i = 0; i < 8; ++i) {
+      float* p = part[i / kChain];
+      if (i % kChain == 0) mma_16816_first(Op(), p, a[i / 4][i % 4], b[i / 4] + 2 * (i % 4));
+      else mma_16816(Op(), p, a[i / 4][i % 4], b[i / 4] + 2 * (i % 4));
+    }
+    if constexpr (GROUP == 128) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int c = t * 8 + g;
-        const uint64_t m = m0 + c / kParts;
-        uint32_t b[8] = {};
-        if (m < rows && c / kParts < kRows) {
-          const T* row = x + m * ld_x + col;
-          load_columns<T, WIDE>(row, c % kParts, b);
-          if (second) load_columns<T, WIDE>(row + 32, c % kParts, b + 4);
-        }
+      for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(part[0][e] + part[1][e], e < 2 ? scale[0].x : scale[0].y, acc[t][e]);
+    } else {
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+      for (int i = 0; i < Weights<GROUP>::kGroups; ++i)
 #pragma unroll
-          for (int h = 0; h < (SHORT ? 2 : 1); ++h) {
-            float part[4] = {};
+        for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(part[i][e], e < 2 ? scale[i].x : scale[i].y, acc[t][e]);
+    }
+  }
+}
+
+// A span of x in shared memory: rows of 128 values whose 16-byte units change
+// places in odd rows, so that the rows g and g + 1 that a quarter warp reads do
+// not meet in a bank.
+template <typename T>
+struct XTile {
+  static constexpr int kUnits = 8 * (int)sizeof(T), kBytes = 128 * (int)sizeof(T);
+  static SVL_DEV int unit(int row, int u) { return row * kUnits + (u ^ (sizeof(T) == 2 ? (row & 1) << 2 : row & 1)); }
+  // A lane's 8 columns of each half of each block, of one row.
+  static SVL_DEV void columns(const uint4* from, int row, int q, int part, uint32_t (*b)[8]) {
+    constexpr int kEach = (int)sizeof(T) / 2;  // units of 8 columns
 #pragma unroll
-            for (int s = SHORT ? 2 * h : 0; s < (SHORT ? 2 * h + 2 : 4); ++s) mma_16816(Op(), part, a[r][s], b + 2 * s);
-            const float s0 = scale_of((uint16_t)scale[d][r][h], w.scale_dtype);
-            const float s1 = scale_of((uint16_t)(scale[d][r][h] >> 16), w.scale_dtype);
-            acc[r][t][0] = fmaf(part[0], s0, acc[r][t][0]);
-            acc[r][t][1] = fmaf(part[1], s0, acc[r][t][1]);
-            acc[r][t][2] = fmaf(part[2], s1, acc[r][t][2]);
-            acc[r][t][3] = fmaf(part[3], s1, acc[r][t][3]);
-          }
+    for (int h = 0; h < 4; ++h) {
+      uint4 v[kEach];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) v[i] = from[unit(row, (h * 4 + q) * kEach + i)];
+      pack_columns<T>(v, part, b[h >> 1] + 4 * (h & 1));
+    }
+  }
+  // The same from global memory; columns behind the matrix are zero (k is a multiple of 32).
+  static SVL_DEV void columns(const T* row, uint32_t col0, uint32_t k, int q, int part, uint32_t (*b)[8]) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      uint32_t* to = b[h >> 1] + 4 * (h & 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to[i] = 0;
+      if (col0 + 32 * h < k) load_columns<T>(row + col0 + 32 * h + 8 * q, part, to);
+    }
+  }
+};
+
+// Copies by threads `tid` of N of spans of up to ROWS rows of x, one after
+// another from `first` on.
+template <typename T, int ROWS, int N>
+struct XCopies {
+  static constexpr int kUnits = XTile<T>::kUnits, kStep = N / kUnits, kCopies = (ROWS + kStep - 1) / kStep;
+  static_assert(kStep % 2 == 0 || kStep == 1, "a thread's rows are all even or all odd, or alternate");
+  const T *from, *x;
+  uint64_t stride;
+  uint32_t col, k, to;
+  int row, rows;
+  SVL_DEV XCopies(const T* x_, uint64_t ld, int rows_, uint32_t first, uint32_t k_, int tid) {
+    const int u = tid % kUnits;
+    x = x_;
+    row = tid / kUnits;
+    rows = rows_;
+    k = k_;
+    col = first * 128 + u * (16 / (int)sizeof(T));
+    from = x + row * ld + col;
+    stride = kStep * ld;
+    to = XTile<T>::unit(row, u) * 16;
+  }
+  SVL_DEV void copy(uint32_t smem, int i) const {
+    const bool there = col + i * 128 < k;
+    const T* src = there ? from + i * 128 : x;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      if (row + c * kStep < rows) {
+        // a step of one row changes the order of its units (FP32: neighbours)
+        const uint32_t flip = kStep == 1 ? (c & 1) * 16 : 0;
+        copy16(smem + (to ^ flip) + c * kStep * XTile<T>::kBytes, there ? src + c * stride : x, there);
       }
     }
   }
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float* to = sums + ((warp * R + r) * 16 + g) * kCols + t * 8 + 2 * q;
-      *(float2*)to = make_float2(acc[r][t][0], acc[r][t][1]);
-      *(float2*)(to + 8 * kCols) = make_float2(acc[r][t][2], acc[r][t][3]);
+  SVL_DEV void advance(int spans) {
+    from += spans * 128;
+    col += spans * 128;
+  }
+};
+
+// Up to 16 columns (rows of x, or parts of them).  One block: 8 / split row
+// blocks; `split` warps share one, take a run of its spans each and join their
+// sums in shared memory, in a fixed order.  Each warp copies its own weights and
+// rows of x ahead, so no barrier stands between load and product.  Tile columns
+// behind the rows repeat the last one and are not written.  WIDE: x has rows of
+// 16-byte units.
+constexpr int kWarpStages = 4;
+template <typename T, int NT, int GROUP, bool HALF, bool ZEROS, bool WIDE>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
+    q4_few_kernel(const __grid_constant__ Q4Matrix w, const T* __restrict__ x, uint64_t ld_x, uint32_t rows,
+                  T* __restrict__ y, uint64_t ld_y, const uint32_t split) {
+  using Op = typename Operand<T>::Type;
+  constexpr int kParts = Operand<T>::kParts, kCols = NT * 8;
+  extern __shared__ __align__(128) uint8_t shared[];
+  float* sums = (float*)shared;  // [warp][16][kCols], after the products
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const uint32_t stage_bytes = sizeof(Weights<GROUP>) + (WIDE ? rows * XTile<T>::kBytes : 0);
+  const uint8_t* ring = shared + (size_t)warp * kWarpStages * stage_bytes;
+  const uint32_t ring_at = smem_u32(ring), spans = w.spans();
+  const uint32_t rb = blockIdx.x * (kWarps / split) + warp / split, turn = warp % split;
+  const bool mine = rb < w.row_blocks();
+  const uint32_t first = (uint32_t)((uint64_t)spans * turn / split);
+  const int count = mine ? (int)((uint64_t)spans * (turn + 1) / split) - (int)first : 0;
+  float acc[NT][4] = {};
+
+  WeightCopies<GROUP, ZEROS> weights(w, mine ? rb : 0, first, lane);
+  XCopies<T, NT * 8 / kParts, 32> columns(x, ld_x, (int)rows, first, w.k, lane);
+  // span `i` from where the copies stand, into a stage
+  auto fetch = [&](int i, int stage, bool in) {
+    if (in) {
+      const uint32_t to = ring_at + stage * stage_bytes;
+      weights.copy(to + lane * 16, i, lane);
+      if (WIDE) columns.copy(to + sizeof(Weights<GROUP>), i);
     }
+    copies_commit();  // also empty: the count of groups in flight stays
+  };
+#pragma unroll
+  for (int i = 0; i < kWarpStages - 1; ++i) fetch(i, i, i < count);
+  int row[NT], part[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    row[t] = min((t * 8 + g) / kParts, (int)rows - 1);
+    part[t] = (t * 8 + g) % kParts;
+  }
+#pragma unroll 1
+  for (int i = 0; i < count; i += kWarpStages) {
+#pragma unroll
+    for (int u = 0; u < kWarpStages; ++u) {
+      if (i + u >= count) break;
+      copies_wait<kWarpStages - 2>();
+      __syncwarp();
+      // into the stage that every lane read a turn ago
+      fetch(u + kWarpStages - 1, (u + kWarpStages - 1) % kWarpStages, i + u + kWarpStages - 1 < count);
+      const uint8_t* st = ring + u * stage_bytes;
+      multiply_span<Op, GROUP, HALF, ZEROS, NT>(acc, *(const Weights<GROUP>*)st, lane, [&](int t, uint32_t(*b)[8]) {
+        if constexpr (WIDE) XTile<T>::columns((const uint4*)(st + sizeof(Weights<GROUP>)), row[t], q, part[t], b);
+        else XTile<T>::columns(x + row[t] * ld_x, (first + i + u) * 128, w.k, q, part[t], b);
+      });
+    }
+    weights.advance(kWarpStages);
+    columns.advance(kWarpStages);
+  }
+  copies_wait<0>();
+  __syncthreads();  // the rings' memory becomes the sums'
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    float* s = sums + (warp * 16 + g) * kCols + t * 8 + 2 * q;
+    *(float2*)s = make_float2(acc[t][0], acc[t][1]);
+    *(float2*)(s + 8 * kCols) = make_float2(acc[t][2], acc[t][3]);
+  }
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * R * kRows; i += kWarps * 32) {
-    const int row = i % (16 * R), c = i / (16 * R);
-    const uint64_t n = (uint64_t)rb0 * 16 + row, m = m0 + c;
-    if (n >= w.n || m >= rows) continue;
+  const int block_rows = 16 * (kWarps / split);
+  for (int i = threadIdx.x; i < block_rows * (int)rows; i += kWarps * 32) {
+    const int r = i % block_rows, m = i / block_rows;
+    const uint64_t n = (uint64_t)blockIdx.x * block_rows + r;
+    if (n >= w.n) continue;
+    const float* from = sums + (r / 16 * split * 16 + r % 16) * kCols + m * kParts;
     float sum = 0.0f;
 #pragma unroll
-    for (int part = kParts - 1; part >= 0; --part)  // the smallest first
-#pragma unroll
-      for (int v = 0; v < kWarps; ++v) sum += sums[(v * R * 16 + row) * kCols + c * kParts + part];
+    for (int p = kParts - 1; p >= 0; --p)  // the smallest first
+      for (uint32_t v = 0; v < split; ++v) sum += from[v * 16 * kCols + p];
     y[m * ld_y + n] = narrow<T>(sum);
   }
+}
+
+// More columns: the 8 warps take different row blocks of the same span, whose
+// rows of x they share; the blocks of a cluster take a run of the spans each and
+// join their sums through each other's shared memory, in a fixed order.
+constexpr int kBlockStages = 3;
+template <typename T, int NT, int GROUP, bool HALF, bool ZEROS>
+__global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 1)
+    q4_many_kernel(const __grid_constant__ Q4Matrix w, const T* __restrict__ x, uint64_t ld_x, uint64_t rows,
+                   T* __restrict__ y, uint64_t ld_y) {
+  using Op = typename Operand<T>::Type;
+  constexpr int kParts = Operand<T>::kParts, kCols = NT * 8, kRows = kCols / kParts, kBlockRows = 16 * kWarps;
+  constexpr uint32_t kStage = kWarps * sizeof(Weights<GROUP>) + kRows * XTile<T>::kBytes;
+  extern __shared__ __align__(128) uint8_t shared[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const uint32_t split = gridDim.z, turn = blockIdx.z;
+  const uint64_t m0 = (uint64_t)blockIdx.y * kRows;
+  const int rows_here = (int)min((uint64_t)kRows, rows - m0);
+  const uint32_t rb = blockIdx.x * kWarps + warp;
+  const bool mine = rb < w.row_blocks();
+  const uint32_t first = (uint32_t)((uint64_t)w.spans() * turn / split);
+  const int count = (int)((uint64_t)w.spans() * (turn + 1) / split) - (int)first;
+  float acc[NT][4] = {};
+
+  WeightCopies<GROUP, ZEROS> weights(w, mine ? rb : 0, first, lane);
+  XCopies<T, kRows, kWarps * 32> columns(x + m0 * ld_x, ld_x, rows_here, first, w.k, threadIdx.x);
+  auto fetch = [&](int stage, bool in) {
+    if (in) {
+      const uint32_t to = smem_u32(shared) + stage * kStage;
+      if (mine) weights.copy(to + warp * sizeof(Weights<GROUP>) + lane * 16, 0, lane);
+      columns.copy(to + kWarps * sizeof(Weights<GROUP>), 0);
+      weights.advance(1);
+      columns.advance(1);
+    }
+    copies_commit();
+  };
+  for (int i = 0; i < kBlockStages - 1; ++i) fetch(i, i < count);
+
+#pragma unroll 1
+  for (int i = 0; i < count; ++i) {
+    const uint8_t* st = shared + i % kBlockStages * kStage;
+    copies_wait<kBlockStages - 2>();
+    __syncthreads();  // everyone's copies of this stage are there, and everyone is done with the one before
+    fetch((i + kBlockStages - 1) % kBlockStages, i + kBlockStages - 1 < count);
+    if (!mine) continue;
+    multiply_span<Op, GROUP, HALF, ZEROS, NT>(
+        acc, ((const Weights<GROUP>*)st)[warp], lane, [&](int t, uint32_t(*b)[8]) {
+          const int c = t * 8 + g, m = min(c / kParts, rows_here - 1);
+          XTile<T>::columns((const uint4*)(st + kWarps * sizeof(Weights<GROUP>)), m, q, c % kParts, b);
+        });
+  }
+  copies_wait<0>();
+  __syncthreads();
+  // [column][row]
+  constexpr int kStride = kBlockRows + 4;
+  float* sums = (float*)shared;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[(t * 8 + 2 * q + (e & 1)) * kStride + warp * 16 + g + 8 * (e >> 1)] = acc[t][e];
+  if (split > 1) cluster_sync();
+  else __syncthreads();
+  // the blocks of the cluster share out the rows
+  const int share = kBlockRows / split, from = turn * share;
+  for (int i = threadIdx.x; i < share * rows_here; i += kWarps * 32) {
+    const int row = from + i % share, m = i / share;
+    const uint64_t n = (uint64_t)blockIdx.x * kBlockRows + row;
+    if (n >= w.n) continue;
+    float sum = 0.0f;
+#pragma unroll
+    for (int part = kParts - 1; part >= 0; --part)
+      for (uint32_t v = 0; v < split; ++v) {
+        const float* s = sums + (m * kParts + part) * kStride + row;
+        float value;
+        if (split == 1) value = *s;
+        else asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(value) : "r"(map_to_rank(smem_u32(s), v)) : "memory");
+        sum += value;
+      }
+    y[(m0 + m) * ld_y + n] = narrow<T>(sum);
+  }
+  if (split > 1) cluster_sync();  // no block leaves while another reads its sums
 }
 
 // One warp per group: its range, scale, zero and codes.
@@ -385,8 +644,8 @@ int q4_reserve(svl_q4* w, int device, uint32_t n, uint32_t k, uint32_t group, ui
   w->m.group = group;
   w->m.scale_dtype = scale_dtype;
   const uint64_t rb = w->m.row_blocks();
-  const size_t codes = rb * w->m.col_blocks() * 512, pairs = rb * w->m.groups() * 8;
-  const cudaError_t e = cudaMalloc(&w->block, codes + pairs * 4 + (zeros ? pairs * 2 : 0));
+  const size_t codes = rb * w->m.spans() * 1024, pairs = rb * w->m.spans() * w->m.span_groups() * 8;
+  const cudaError_t e = cudaMalloc(&w->block, codes + pairs * 4 + (zeros ? pairs : 0));
   if (e != cudaSuccess) {
     w->block = nullptr;
     return svl::cuda_failure(e, err, err_len);
@@ -394,7 +653,7 @@ int q4_reserve(svl_q4* w, int device, uint32_t n, uint32_t k, uint32_t group, ui
   uint8_t* p = (uint8_t*)w->block;
   w->m.codes = (const uint4*)p;
   w->m.scales = (const uint32_t*)(p + codes);
-  w->m.zeros = zeros ? (const uint16_t*)(p + codes + pairs * 4) : nullptr;
+  w->m.zeros = zeros ? p + codes + pairs * 4 : nullptr;
   return SVL_OK;
 }
 
@@ -413,54 +672,111 @@ cudaError_t on_device(const void* src, size_t bytes, int device, svl::Freed& hel
 }
 
 cudaError_t lay_out(const svl_q4& w, const void* codes, const void* scales, const void* zeros) {
-  const uint64_t words = (uint64_t)w.m.row_blocks() * w.m.col_blocks() * 128;
+  const uint64_t words = (uint64_t)w.m.row_blocks() * w.m.spans() * 256;
   svl::q4_lay_out_kernel<<<(unsigned)std::min<uint64_t>((words + 255) / 256, 148 * 8), 256>>>(
       w.m, (const uint8_t*)codes, (const uint16_t*)scales, (const uint8_t*)zeros);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? cudaStreamSynchronize(nullptr) : e;
 }
 
-template <typename T, int NT, int R, bool SHORT, bool WIDE>
-cudaError_t launch_rows(const svl::Q4Matrix& m, const void* x, uint64_t ld_x, uint64_t rows, void* y, uint64_t ld_y,
-                        cudaStream_t st) {
-  constexpr uint32_t kRows = NT * 8 / svl::Operand<T>::kParts;
-  constexpr int smem = svl::kWarps * R * 16 * NT * 8 * 4;
+constexpr uint32_t kSms = 148;
+
+struct Rows {
+  const void* x;
+  uint64_t ld_x, rows;
+  void* y;
+  uint64_t ld_y;
+};
+
+template <typename T, int NT, int GROUP, bool HALF, bool ZEROS, bool WIDE>
+cudaError_t launch_few(const svl::Q4Matrix& m, const Rows& r, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  auto kernel = svl::q4_linear_kernel<T, NT, R, SHORT, WIDE>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = smem_opt_in(kernel, smem, &done);
-    if (e != cudaSuccess) return e;
-  }
-  // a grid's second dimension ends at 65535
-  for (uint64_t m0 = 0; m0 < rows; m0 += 65535ull * kRows) {
-    const uint64_t now = std::min<uint64_t>(rows - m0, 65535ull * kRows);
-    const dim3 grid((m.row_blocks() + R - 1) / R, (unsigned)((now + kRows - 1) / kRows));
-    kernel<<<grid, svl::kWarps * 32, smem, st>>>(m, (const T*)x + m0 * ld_x, ld_x, now, (T*)y + m0 * ld_y, ld_y);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
+  auto kernel = svl::q4_few_kernel<T, NT, GROUP, HALF, ZEROS, WIDE>;
+  constexpr uint32_t kMost = NT * 8 / svl::Operand<T>::kParts;
+  auto smem = [](uint64_t n) {
+    const size_t stage = sizeof(svl::Weights<GROUP>) + (WIDE ? n * svl::XTile<T>::kBytes : 0);
+    return svl::kWarps * (int)std::max<size_t>(svl::kWarpStages * stage, 16 * NT * 8 * 4);
+  };
+  const cudaError_t e = smem_opt_in(kernel, smem(kMost), &done);
+  if (e != cudaSuccess) return e;
+  // Warps to a row block: as many as leave each a run of four spans, more where
+  // there would not be a block for every SM.
+  uint32_t split = 1;
+  while (split < svl::kWarps && 2 * split <= m.spans() &&
+         (m.spans() >= 8 * split || (uint64_t)m.row_blocks() * split < (uint64_t)kSms * svl::kWarps))
+    split *= 2;
+  const uint32_t per_block = svl::kWarps / split;
+  const dim3 grid((m.row_blocks() + per_block - 1) / per_block);
+  // without 16-byte units more rows come here too, so many at a time
+  for (uint64_t m0 = 0; m0 < r.rows; m0 += kMost) {
+    const uint32_t now = (uint32_t)std::min<uint64_t>(r.rows - m0, kMost);
+    kernel<<<grid, svl::kWarps * 32, smem(now), st>>>(m, (const T*)r.x + m0 * r.ld_x, r.ld_x, now, (T*)r.y + m0 * r.ld_y,
+                                                      r.ld_y, split);
+    const cudaError_t f = cudaGetLastError();
+    if (f != cudaSuccess) return f;
   }
   return cudaSuccess;
 }
 
-template <typename T, bool SHORT, bool WIDE>
-cudaError_t launch_linear(const svl::Q4Matrix& m, const void* x, uint64_t ld_x, uint64_t rows, void* y, uint64_t ld_y,
-                          cudaStream_t st) {
-  const uint64_t cols = rows * svl::Operand<T>::kParts;
-  if (cols <= 8) return launch_rows<T, 1, 1, SHORT, WIDE>(m, x, ld_x, rows, y, ld_y, st);
-  if (cols <= 16) return launch_rows<T, 2, 1, SHORT, WIDE>(m, x, ld_x, rows, y, ld_y, st);
-  if (cols <= 32) return launch_rows<T, 4, 1, SHORT, WIDE>(m, x, ld_x, rows, y, ld_y, st);
-  return launch_rows<T, 8, 2, SHORT, WIDE>(m, x, ld_x, rows, y, ld_y, st);
+template <typename T, int NT, int GROUP, bool HALF, bool ZEROS>
+cudaError_t launch_many(const svl::Q4Matrix& m, const Rows& r, cudaStream_t st) {
+  constexpr uint32_t kRows = NT * 8 / svl::Operand<T>::kParts, kBlockRows = 16 * svl::kWarps;
+  constexpr int ring = svl::kBlockStages * (svl::kWarps * (int)sizeof(svl::Weights<GROUP>) + kRows * svl::XTile<T>::kBytes);
+  constexpr int sums = NT * 8 * (kBlockRows + 4) * 4, smem = ring > sums ? ring : sums;
+  static std::atomic<uint64_t> done{0};
+  auto kernel = svl::q4_many_kernel<T, NT, GROUP, HALF, ZEROS>;
+  const cudaError_t e = smem_opt_in(kernel, smem, &done);
+  if (e != cudaSuccess) return e;
+  const uint32_t units = (m.row_blocks() + svl::kWarps - 1) / svl::kWarps;
+  const uint64_t slabs = (r.rows + kRows - 1) / kRows;
+  // Blocks of a cluster: up to 8, while all of them run at once and each has
+  // two spans.
+  uint32_t split = 1;
+  while (split < 8 && split * 4 <= m.spans() && units * slabs * split * 2 <= kSms) split *= 2;
+  // a grid's second dimension ends at 65535
+  for (uint64_t m0 = 0; m0 < r.rows; m0 += 65535ull * kRows) {
+    const uint64_t now = std::min<uint64_t>(r.rows - m0, 65535ull * kRows);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(units, (unsigned)((now + kRows - 1) / kRows), split);
+    cfg.blockDim = dim3(svl::kWarps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = split;
+    cfg.attrs = attr;
+    cfg.numAttrs = split > 1 ? 1 : 0;
+    const cudaError_t f = cudaLaunchKernelEx(&cfg, kernel, m, (const T*)r.x + m0 * r.ld_x, r.ld_x, now,
+                                             (T*)r.y + m0 * r.ld_y, r.ld_y);
+    if (f != cudaSuccess) return f;
+  }
+  return cudaSuccess;
+}
+
+template <typename T, int GROUP, bool HALF, bool ZEROS>
+cudaError_t launch_rows(const svl::Q4Matrix& m, const Rows& r, cudaStream_t st) {
+  constexpr uint64_t kParts = svl::Operand<T>::kParts;
+  if (((uintptr_t)r.x | r.ld_x * sizeof(T)) % 16) return launch_few<T, 2, GROUP, HALF, ZEROS, false>(m, r, st);
+  if (r.rows <= 8 / kParts) return launch_few<T, 1, GROUP, HALF, ZEROS, true>(m, r, st);
+  if (r.rows <= 16 / kParts) return launch_few<T, 2, GROUP, HALF, ZEROS, true>(m, r, st);
+  if (r.rows <= 32 / kParts) return launch_many<T, 4, GROUP, HALF, ZEROS>(m, r, st);
+  return launch_many<T, 8, GROUP, HALF, ZEROS>(m, r, st);
+}
+
+template <typename T, int GROUP>
+cudaError_t launch_group(const svl::Q4Matrix& m, const Rows& r, cudaStream_t st) {
+  const bool half = m.scale_dtype == SVL_DTYPE_F16;
+  if (m.zeros) return half ? launch_rows<T, GROUP, true, true>(m, r, st) : launch_rows<T, GROUP, false, true>(m, r, st);
+  return half ? launch_rows<T, GROUP, true, false>(m, r, st) : launch_rows<T, GROUP, false, false>(m, r, st);
 }
 
 template <typename T>
-cudaError_t launch_linear(const svl::Q4Matrix& m, const void* x, uint64_t ld_x, uint64_t rows, void* y, uint64_t ld_y,
-                          cudaStream_t st) {
-  const bool wide = ((uintptr_t)x | ld_x * sizeof(T)) % 16 == 0;
-  if (m.group == 32)
-    return wide ? launch_linear<T, true, true>(m, x, ld_x, rows, y, ld_y, st)
-                : launch_linear<T, true, false>(m, x, ld_x, rows, y, ld_y, st);
-  return wide ? launch_linear<T, false, true>(m, x, ld_x, rows, y, ld_y, st)
-              : launch_linear<T, false, false>(m, x, ld_x, rows, y, ld_y, st);
+cudaError_t launch_linear(const svl::Q4Matrix& m, const Rows& r, cudaStream_t st) {
+  return m.group == 32   ? launch_group<T, 32>(m, r, st)
+         : m.group == 64 ? launch_group<T, 64>(m, r, st)
+                         : launch_group<T, 128>(m, r, st);
 }
 
 }  // namespace
@@ -580,9 +896,10 @@ int svl_q4_linear_device(const svl_q4* weight, uint32_t dtype, const void* d_x, 
   svl::DeviceGuard on(weight->device);
   if (on.status != cudaSuccess) return svl::cuda_failure(on.status, err, err_len);
   cudaStream_t st = (cudaStream_t)stream;
-  const cudaError_t e = dtype == SVL_DTYPE_F32    ? launch_linear<float>(m, d_x, ld_x, rows, d_y, ld_y, st)
-                        : dtype == SVL_DTYPE_BF16 ? launch_linear<__nv_bfloat16>(m, d_x, ld_x, rows, d_y, ld_y, st)
-                                                  : launch_linear<__half>(m, d_x, ld_x, rows, d_y, ld_y, st);
+  const Rows r{d_x, ld_x, rows, d_y, ld_y};
+  const cudaError_t e = dtype == SVL_DTYPE_F32    ? launch_linear<float>(m, r, st)
+                        : dtype == SVL_DTYPE_BF16 ? launch_linear<__nv_bfloat16>(m, r, st)
+                                                  : launch_linear<__half>(m, r, st);
   return e == cudaSuccess ? SVL_OK : svl::cuda_failure(e, err, err_len);
 }
 

@@ -19,6 +19,7 @@ it.
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import numpy as np
 
@@ -67,6 +68,16 @@ def _whole(values, dtype, what: str) -> np.ndarray:
 
 def _ptr(a):
     return None if a is None else a.ctypes.data
+
+
+class _PerThread(threading.local):
+    """One message buffer a thread for the calls on device buffers, which are short."""
+
+    def __init__(self):
+        self.err = ErrBuf()
+
+
+_thread = _PerThread()
 
 
 class _Handle:
@@ -121,7 +132,7 @@ class AxisRope(_Handle):
                      device: int = 0, stream: int = 0) -> None:
         """Rotates ``n_tokens`` rows of ``q_heads`` and ``k_heads`` heads; ``positions``
         holds ``n_axes`` x ``n_tokens`` int32.  In place where an output is its input."""
-        eb = ErrBuf()
+        eb = _thread.err
         rc = self._lib.svl_rope_apply_device(self._h, device, _dtype(dtype), positions, n_tokens, q, ld_q, q_heads,
                                              q_out, ld_q_out, k, ld_k, k_heads, k_out, ld_k_out, stream or None,
                                              *eb.args)
@@ -181,7 +192,7 @@ class AttentionPlan(_Handle):
     def run_device(self, q: int, ld_q: int, k: int, ld_k: int, v: int, ld_v: int, out: int, ld_out: int, lse: int = 0,
                    workspace: int = 0, workspace_bytes: int = 0, stream: int = 0) -> None:
         """One attention over the batch; ``lse`` (optional): q rows x q_heads float32."""
-        eb = ErrBuf()
+        eb = _thread.err
         rc = self._lib.svl_attention_device(self._h, q, ld_q, k, ld_k, v, ld_v, out, ld_out, lse or None,
                                             workspace or None, workspace_bytes, stream or None, *eb.args)
         if rc:
@@ -241,7 +252,7 @@ class Q4Weight(_Handle):
 
     def linear_device(self, dtype: str, x: int, ld_x: int, rows: int, y: int, ld_y: int, stream: int = 0) -> None:
         """y = x W^T for ``rows`` rows."""
-        eb = ErrBuf()
+        eb = _thread.err
         rc = self._lib.svl_q4_linear_device(self._h, _dtype(dtype), x, ld_x, rows, y, ld_y, stream or None, *eb.args)
         if rc:
             eb.check(rc)
