@@ -204,7 +204,8 @@ SVL_DEV void load_columns(const T* row, int part, uint32_t* b) {
   pack_columns<T>(v, part, b);
 }
 
-// Asynchronous copies to shared memory.  `there` false: 16 zero bytes, nothing is read.
+// Asynchronous copies to shared memory.  `there` false: 16 zero bytes; with a
+// source size of 0 the address is not looked at.
 SVL_DEV void copy16(uint32_t smem, const void* src, bool there = true) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
@@ -324,14 +325,17 @@ template <typename T>
 struct XTile {
   static constexpr int kUnits = 8 * (int)sizeof(T), kBytes = 128 * (int)sizeof(T);
   static SVL_DEV int unit(int row, int u) { return row * kUnits + (u ^ (sizeof(T) == 2 ? (row & 1) << 2 : row & 1)); }
-  // A lane's 8 columns of each half of each block, of one row.
-  static SVL_DEV void columns(const uint4* from, int row, int q, int part, uint32_t (*b)[8]) {
-    constexpr int kEach = (int)sizeof(T) / 2;  // units of 8 columns
+  // A lane's 8 columns of each half of each block, of one row: from byte offset
+  // `even` in the even halves and `odd` in the odd ones.
+  static SVL_DEV uint32_t offset(int row, int q, int half) { return unit(row, (half * 4 + q) * ((int)sizeof(T) / 2)) * 16; }
+  static SVL_DEV void columns(const uint8_t* tile, uint32_t even, uint32_t odd, int part, uint32_t (*b)[8]) {
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      uint4 v[kEach];
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) v[i] = from[unit(row, (h * 4 + q) * kEach + i)];
+      const uint4* from = (const uint4*)(tile + (h & 1 ? odd : even) + (h >> 1) * (kBytes / 2));
+      uint4 v[sizeof(T) / 2];
+      v[0] = from[0];
+      // the neighbour of an FP32 unit is its partner in the row's order
+      if constexpr (sizeof(T) == 4) v[1] = *(const uint4*)((uintptr_t)from ^ 16);
       pack_columns<T>(v, part, b[h >> 1] + 4 * (h & 1));
     }
   }
@@ -353,36 +357,36 @@ template <typename T, int ROWS, int N>
 struct XCopies {
   static constexpr int kUnits = XTile<T>::kUnits, kStep = N / kUnits, kCopies = (ROWS + kStep - 1) / kStep;
   static_assert(kStep % 2 == 0 || kStep == 1, "a thread's rows are all even or all odd, or alternate");
-  const T *from, *x;
+  const T* from;
   uint64_t stride;
-  uint32_t col, k, to;
-  int row, rows;
-  SVL_DEV XCopies(const T* x_, uint64_t ld, int rows_, uint32_t first, uint32_t k_, int tid) {
+  uint32_t to;
+  int row, rows, whole;  // spans from here on that lie inside the matrix
+  bool in_last;          // this thread's unit of the span behind them does
+  SVL_DEV XCopies(const T* x, uint64_t ld, int rows_, uint32_t first, uint32_t k, int tid) {
     const int u = tid % kUnits;
-    x = x_;
     row = tid / kUnits;
     rows = rows_;
-    k = k_;
-    col = first * 128 + u * (16 / (int)sizeof(T));
-    from = x + row * ld + col;
+    from = x + row * ld + first * 128 + u * (16 / (int)sizeof(T));
     stride = kStep * ld;
     to = XTile<T>::unit(row, u) * 16;
+    whole = (int)(k / 128) - (int)first;
+    in_last = u * (16 / (int)sizeof(T)) < (int)(k % 128);
   }
   SVL_DEV void copy(uint32_t smem, int i) const {
-    const bool there = col + i * 128 < k;
-    const T* src = there ? from + i * 128 : x;
+    const bool there = i < whole || in_last;
 #pragma unroll
     for (int c = 0; c < kCopies; ++c) {
+      if (ROWS > 1 && c * kStep >= rows) break;
       if (row + c * kStep < rows) {
         // a step of one row changes the order of its units (FP32: neighbours)
         const uint32_t flip = kStep == 1 ? (c & 1) * 16 : 0;
-        copy16(smem + (to ^ flip) + c * kStep * XTile<T>::kBytes, there ? src + c * stride : x, there);
+        copy16(smem + (to ^ flip) + c * kStep * XTile<T>::kBytes, from + c * stride + i * 128, there);
       }
     }
   }
   SVL_DEV void advance(int spans) {
     from += spans * 128;
-    col += spans * 128;
+    whole -= spans;
   }
 };
 
@@ -392,18 +396,19 @@ struct XCopies {
 // rows of x ahead, so no barrier stands between load and product.  Tile columns
 // behind the rows repeat the last one and are not written.  WIDE: x has rows of
 // 16-byte units.
-constexpr int kWarpStages = 4;
-template <typename T, int NT, int GROUP, bool HALF, bool ZEROS, bool WIDE>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
+constexpr int few_stages(int cols) { return cols <= 8 ? 4 : 2; }  // so that two blocks fit an SM
+template <typename T, int ROWS, int GROUP, bool HALF, bool ZEROS, bool WIDE>
+__global__ void __launch_bounds__(kWarps * 32, ROWS == 1 ? 3 : 2)
     q4_few_kernel(const __grid_constant__ Q4Matrix w, const T* __restrict__ x, uint64_t ld_x, uint32_t rows,
                   T* __restrict__ y, uint64_t ld_y, const uint32_t split) {
   using Op = typename Operand<T>::Type;
-  constexpr int kParts = Operand<T>::kParts, kCols = NT * 8;
+  constexpr int kParts = Operand<T>::kParts, NT = (ROWS * kParts + 7) / 8, kCols = NT * 8;
+  constexpr int kStages = few_stages(ROWS * kParts);
+  constexpr uint32_t kStage = sizeof(Weights<GROUP>) + (WIDE ? ROWS * XTile<T>::kBytes : 0);
   extern __shared__ __align__(128) uint8_t shared[];
   float* sums = (float*)shared;  // [warp][16][kCols], after the products
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const uint32_t stage_bytes = sizeof(Weights<GROUP>) + (WIDE ? rows * XTile<T>::kBytes : 0);
-  const uint8_t* ring = shared + (size_t)warp * kWarpStages * stage_bytes;
+  const uint8_t* ring = shared + warp * kStages * kStage;
   const uint32_t ring_at = smem_u32(ring), spans = w.spans();
   const uint32_t rb = blockIdx.x * (kWarps / split) + warp / split, turn = warp % split;
   const bool mine = rb < w.row_blocks();
@@ -412,41 +417,44 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
   float acc[NT][4] = {};
 
   WeightCopies<GROUP, ZEROS> weights(w, mine ? rb : 0, first, lane);
-  XCopies<T, NT * 8 / kParts, 32> columns(x, ld_x, (int)rows, first, w.k, lane);
+  XCopies<T, ROWS, 32> columns(x, ld_x, (int)rows, first, w.k, lane);
   // span `i` from where the copies stand, into a stage
   auto fetch = [&](int i, int stage, bool in) {
     if (in) {
-      const uint32_t to = ring_at + stage * stage_bytes;
+      const uint32_t to = ring_at + stage * kStage;
       weights.copy(to + lane * 16, i, lane);
       if (WIDE) columns.copy(to + sizeof(Weights<GROUP>), i);
     }
     copies_commit();  // also empty: the count of groups in flight stays
   };
 #pragma unroll
-  for (int i = 0; i < kWarpStages - 1; ++i) fetch(i, i, i < count);
+  for (int i = 0; i < kStages - 1; ++i) fetch(i, i, i < count);
   int row[NT], part[NT];
+  uint32_t even[NT], odd[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    row[t] = min((t * 8 + g) / kParts, (int)rows - 1);
+    row[t] = ROWS == 1 ? 0 : min((t * 8 + g) / kParts, (int)rows - 1);
     part[t] = (t * 8 + g) % kParts;
+    even[t] = sizeof(Weights<GROUP>) + XTile<T>::offset(row[t], q, 0);
+    odd[t] = ROWS == 1 ? even[t] + XTile<T>::kBytes / 4 : sizeof(Weights<GROUP>) + XTile<T>::offset(row[t], q, 1);
   }
 #pragma unroll 1
-  for (int i = 0; i < count; i += kWarpStages) {
+  for (int i = 0; i < count; i += kStages) {
 #pragma unroll
-    for (int u = 0; u < kWarpStages; ++u) {
+    for (int u = 0; u < kStages; ++u) {
       if (i + u >= count) break;
-      copies_wait<kWarpStages - 2>();
+      copies_wait<kStages - 2>();
       __syncwarp();
       // into the stage that every lane read a turn ago
-      fetch(u + kWarpStages - 1, (u + kWarpStages - 1) % kWarpStages, i + u + kWarpStages - 1 < count);
-      const uint8_t* st = ring + u * stage_bytes;
+      fetch(u + kStages - 1, (u + kStages - 1) % kStages, i + u + kStages - 1 < count);
+      const uint8_t* st = ring + u * kStage;
       multiply_span<Op, GROUP, HALF, ZEROS, NT>(acc, *(const Weights<GROUP>*)st, lane, [&](int t, uint32_t(*b)[8]) {
-        if constexpr (WIDE) XTile<T>::columns((const uint4*)(st + sizeof(Weights<GROUP>)), row[t], q, part[t], b);
+        if constexpr (WIDE) XTile<T>::columns(st, even[t], odd[t], part[t], b);
         else XTile<T>::columns(x + row[t] * ld_x, (first + i + u) * 128, w.k, q, part[t], b);
       });
     }
-    weights.advance(kWarpStages);
-    columns.advance(kWarpStages);
+    weights.advance(kStages);
+    columns.advance(kStages);
   }
   copies_wait<0>();
   __syncthreads();  // the rings' memory becomes the sums'
@@ -517,7 +525,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 1)
     multiply_span<Op, GROUP, HALF, ZEROS, NT>(
         acc, ((const Weights<GROUP>*)st)[warp], lane, [&](int t, uint32_t(*b)[8]) {
           const int c = t * 8 + g, m = min(c / kParts, rows_here - 1);
-          XTile<T>::columns((const uint4*)(st + kWarps * sizeof(Weights<GROUP>)), m, q, c % kParts, b);
+          XTile<T>::columns(st + kWarps * sizeof(Weights<GROUP>), XTile<T>::offset(m, q, 0), XTile<T>::offset(m, q, 1),
+                            c % kParts, b);
         });
   }
   copies_wait<0>();
@@ -688,16 +697,15 @@ struct Rows {
   uint64_t ld_y;
 };
 
-template <typename T, int NT, int GROUP, bool HALF, bool ZEROS, bool WIDE>
+template <typename T, int ROWS, int GROUP, bool HALF, bool ZEROS, bool WIDE>
 cudaError_t launch_few(const svl::Q4Matrix& m, const Rows& r, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  auto kernel = svl::q4_few_kernel<T, NT, GROUP, HALF, ZEROS, WIDE>;
-  constexpr uint32_t kMost = NT * 8 / svl::Operand<T>::kParts;
-  auto smem = [](uint64_t n) {
-    const size_t stage = sizeof(svl::Weights<GROUP>) + (WIDE ? n * svl::XTile<T>::kBytes : 0);
-    return svl::kWarps * (int)std::max<size_t>(svl::kWarpStages * stage, 16 * NT * 8 * 4);
-  };
-  const cudaError_t e = smem_opt_in(kernel, smem(kMost), &done);
+  auto kernel = svl::q4_few_kernel<T, ROWS, GROUP, HALF, ZEROS, WIDE>;
+  constexpr int cols = ROWS * svl::Operand<T>::kParts;
+  constexpr int stage = (int)sizeof(svl::Weights<GROUP>) + (WIDE ? ROWS * svl::XTile<T>::kBytes : 0);
+  constexpr int ring = svl::few_stages(cols) * stage, sums = 16 * ((cols + 7) / 8) * 8 * 4;
+  constexpr int smem = svl::kWarps * (ring > sums ? ring : sums);
+  const cudaError_t e = smem_opt_in(kernel, smem, &done);
   if (e != cudaSuccess) return e;
   // Warps to a row block: as many as leave each a run of four spans, more where
   // there would not be a block for every SM.
@@ -708,9 +716,9 @@ cudaError_t launch_few(const svl::Q4Matrix& m, const Rows& r, cudaStream_t st) {
   const uint32_t per_block = svl::kWarps / split;
   const dim3 grid((m.row_blocks() + per_block - 1) / per_block);
   // without 16-byte units more rows come here too, so many at a time
-  for (uint64_t m0 = 0; m0 < r.rows; m0 += kMost) {
-    const uint32_t now = (uint32_t)std::min<uint64_t>(r.rows - m0, kMost);
-    kernel<<<grid, svl::kWarps * 32, smem(now), st>>>(m, (const T*)r.x + m0 * r.ld_x, r.ld_x, now, (T*)r.y + m0 * r.ld_y,
+  for (uint64_t m0 = 0; m0 < r.rows; m0 += ROWS) {
+    const uint32_t now = (uint32_t)std::min<uint64_t>(r.rows - m0, ROWS);
+    kernel<<<grid, svl::kWarps * 32, smem, st>>>(m, (const T*)r.x + m0 * r.ld_x, r.ld_x, now, (T*)r.y + m0 * r.ld_y,
                                                       r.ld_y, split);
     const cudaError_t f = cudaGetLastError();
     if (f != cudaSuccess) return f;
@@ -757,10 +765,11 @@ cudaError_t launch_many(const svl::Q4Matrix& m, const Rows& r, cudaStream_t st) 
 
 template <typename T, int GROUP, bool HALF, bool ZEROS>
 cudaError_t launch_rows(const svl::Q4Matrix& m, const Rows& r, cudaStream_t st) {
-  constexpr uint64_t kParts = svl::Operand<T>::kParts;
-  if (((uintptr_t)r.x | r.ld_x * sizeof(T)) % 16) return launch_few<T, 2, GROUP, HALF, ZEROS, false>(m, r, st);
-  if (r.rows <= 8 / kParts) return launch_few<T, 1, GROUP, HALF, ZEROS, true>(m, r, st);
-  if (r.rows <= 16 / kParts) return launch_few<T, 2, GROUP, HALF, ZEROS, true>(m, r, st);
+  constexpr int kParts = svl::Operand<T>::kParts;
+  if (((uintptr_t)r.x | r.ld_x * sizeof(T)) % 16) return launch_few<T, 16 / kParts, GROUP, HALF, ZEROS, false>(m, r, st);
+  if (r.rows == 1) return launch_few<T, 1, GROUP, HALF, ZEROS, true>(m, r, st);
+  if (r.rows <= 8 / kParts) return launch_few<T, 8 / kParts, GROUP, HALF, ZEROS, true>(m, r, st);
+  if (r.rows <= 16 / kParts) return launch_few<T, 16 / kParts, GROUP, HALF, ZEROS, true>(m, r, st);
   if (r.rows <= 32 / kParts) return launch_many<T, 4, GROUP, HALF, ZEROS>(m, r, st);
   return launch_many<T, 8, GROUP, HALF, ZEROS>(m, r, st);
 }
