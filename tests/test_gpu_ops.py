@@ -26,6 +26,12 @@ def half_step(dtype):
     return torch.finfo(TYPES[dtype]).eps / 2
 
 
+def least_half_step(dtype):
+    """Half the spacing of the type's smallest values (FP16: 2^-24 below 2^-14), where half_step is no longer relative."""
+    info = torch.finfo(TYPES[dtype])
+    return info.eps * info.tiny / 2
+
+
 def stream():
     return torch.cuda.current_stream().cuda_stream
 
@@ -70,7 +76,7 @@ def rope_tolerance(dtype, y, size, far):
     # the angle in half turns is rounded to FP32 (2^-25 of a half turn: 3.2 2^-25 rad, under 2 2^-24), sine and
     # cosine are within 2 units, two products and a sum round: 6 2^-24 of |x| + |y| in all; the 64-bit reference's own
     # angle is off by far * 2^-53 (its product's rounding) and as much for its frequency
-    return size * (6 * 2.0 ** -24 + far * 2.0 ** -52) + half_step(dtype) * y.abs()
+    return size * (6 * 2.0 ** -24 + far * 2.0 ** -52) + half_step(dtype) * y.abs() + least_half_step(dtype)
 
 
 def run_rope(dtype, tokens, qh, kh, hd, pairs, arrangement, far=0, pad=0, offset=0, in_place=False, seed=0, theta=None):
@@ -104,7 +110,7 @@ def run_rope(dtype, tokens, qh, kh, hd, pairs, arrangement, far=0, pad=0, offset
 @pytest.mark.parametrize("tokens,qh,kh,hd,pairs", [
     (1, 1, 1, 2, [1]), (33, 4, 2, 256, [128]), (17, 16, 16, 72, [18, 18]), (130, 16, 4, 128, [24, 20, 20]),
     (5, 3, 1, 66, [3, 7, 2, 5]), (9, 2, 2, 67, [11, 5]), (3, 1, 1, 512, [100, 156]), (64, 5, 0, 80, [16, 24]),
-    (70, 0, 7, 96, [40]),
+    (70, 0, 7, 96, [40]), (4, 1, 2, 512, [1]), (700, 2, 1, 128, [20, 44]),
 ])
 def test_rope(dtype, arrangement, tokens, qh, kh, hd, pairs):
     run_rope(dtype, tokens, qh, kh, hd, pairs, arrangement)
@@ -163,7 +169,7 @@ def run_linear(dtype, rows, n, k, group, zeros, scale_dtype="bf16", pad=0, offse
     with np.errstate(invalid="ignore"):
         want, size = xs @ full.T, np.abs(xs) @ np.abs(full).T
         # k products summed, the group's sum scaled (one more rounding each), and y rounded
-        bound = (k + k // group + 2) * ULP * size + half_step(dtype) * np.abs(want)
+        bound = (k + k // group + 2) * ULP * size + half_step(dtype) * np.abs(want) + least_half_step(dtype)
         good = np.ones(rows, bool)
         if spoil is not None:
             good[spoil[0]] = False
