@@ -241,7 +241,7 @@ struct svl_attention_plan {
   svl::AttnParams p{};
   int device = -1;
   uint32_t dtype = 0;
-  bool tensor_cores = false;
+  enum Kernel { kGeneral, kTiles, kRows } kernel = kGeneral;
   uint32_t max_join_rows = 0;
   uint64_t workspace = 0;
   void* block = nullptr;
@@ -527,11 +527,20 @@ int svl_attention_plan_create(int device, const svl_attention_config* config, co
     int sms = 0;
     cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e != cudaSuccess) return svl::cuda_failure(e, err, err_len);
-    plan->tensor_cores = svl::attention_tc_takes(c, cu_q[batch], cu_k[batch]);
-    const uint32_t tile_rows = plan->tensor_cores ? svl::attention_tc_tile_rows(group) : svl::kGenRows;
-    const uint32_t row_tiles = plan->tensor_cores ? svl::attention_tc_row_tiles(c.head_dim) : 1;
-    const Schedule s = schedule(c, cu_q, cu_k, batch, prefix, doc_q, doc_k, tile_rows, row_tiles,
-                                (uint32_t)sms * (plan->tensor_cores ? 1 : kGeneralBlocksPerSm));
+    uint32_t tile_rows = svl::kGenRows, row_tiles = 1, per_sm = kGeneralBlocksPerSm;
+    if (svl::attention_tc_takes(c, cu_q[batch], cu_k[batch])) {
+      uint64_t most = 0;
+      for (uint32_t b = 0; b < batch; ++b) most = std::max(most, (cu_q[b + 1] - cu_q[b]) * group);
+      per_sm = 1;
+      plan->kernel = svl_attention_plan::kRows;
+      tile_rows = svl::attention_rows_takes(c.head_dim, most);
+      if (!tile_rows) {
+        plan->kernel = svl_attention_plan::kTiles;
+        tile_rows = svl::attention_tc_tile_rows(group);
+        row_tiles = svl::attention_tc_row_tiles(c.head_dim);
+      }
+    }
+    const Schedule s = schedule(c, cu_q, cu_k, batch, prefix, doc_q, doc_k, tile_rows, row_tiles, (uint32_t)sms * per_sm);
     svl::AttnParams& p = plan->p;
     p.slot_rows = tile_rows * row_tiles;
     // one block of device memory, one copy
@@ -636,7 +645,8 @@ int svl_attention_device(const svl_attention_plan* plan, const void* d_q, uint64
   svl::DeviceGuard on(plan->device);
   if (on.status != cudaSuccess) return svl::cuda_failure(on.status, err, err_len);
   cudaStream_t st = (cudaStream_t)stream;
-  cudaError_t e = plan->tensor_cores              ? svl::attention_tc_launch(p, plan->dtype, st)
+  cudaError_t e = plan->kernel == svl_attention_plan::kRows    ? svl::attention_rows_launch(p, plan->dtype, st)
+                  : plan->kernel == svl_attention_plan::kTiles ? svl::attention_tc_launch(p, plan->dtype, st)
                   : plan->dtype == SVL_DTYPE_F32  ? launch_general<float>(p, st)
                   : plan->dtype == SVL_DTYPE_BF16 ? launch_general<__nv_bfloat16>(p, st)
                                                   : launch_general<__half>(p, st);

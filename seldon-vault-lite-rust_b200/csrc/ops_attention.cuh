@@ -94,5 +94,9 @@ bool attention_tc_takes(const svl_attention_config& c, uint64_t total_q, uint64_
 uint32_t attention_tc_tile_rows(uint32_t group);
 uint32_t attention_tc_row_tiles(uint32_t head_dim);
 cudaError_t attention_tc_launch(const AttnParams& p, uint32_t dtype, cudaStream_t st);
+// The same types with few rows (ops_attention_rows.cu): the rows of a tile that
+// takes a sequence of `rows` (query, head of the group) rows, or 0.
+uint32_t attention_rows_takes(uint32_t head_dim, uint64_t rows);
+cudaError_t attention_rows_launch(const AttnParams& p, uint32_t dtype, cudaStream_t st);
 
 }  // namespace svl

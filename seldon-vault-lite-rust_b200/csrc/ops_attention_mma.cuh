@@ -1,0 +1,98 @@
+// ops_attention_mma.cuh -- what the FP16 / BF16 attention kernels share: the ring
+// of key and value slabs, operand packing, and the care for non-finite values in
+// key tiles that are seen in part.
+#pragma once
+
+#include "ops_attention.cuh"
+
+namespace svl {
+
+// K and V travel in slabs of 128 keys x 64 columns, 128-byte swizzled.
+constexpr int kSlabBytes = 16384, kSlabCols = 64;
+constexpr int kSmemLimit = 232448;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kBehind = 8.0f;  // a maximum follows once it is 2^8 behind (log2 units)
+
+SVL_DEV uint32_t pack2(__half, float lo, float hi) { return pack_half2(lo, hi); }
+SVL_DEV uint32_t pack2(__nv_bfloat16, float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Per packed pair: the sign bit of each half whose exponent is all ones.
+SVL_DEV uint32_t non_finite(__half, uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
+SVL_DEV uint32_t non_finite(__nv_bfloat16, uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+
+struct RingPos {
+  uint32_t stage = 0, phase = 0;
+  template <int N>
+  SVL_DEV void next() {
+    if (++stage == N) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// A position `slabs` further on (less than a turn).
+template <int N>
+SVL_DEV RingPos ahead(RingPos p, uint32_t slabs) {
+  p.stage += slabs;
+  if (p.stage >= N) {
+    p.stage -= N;
+    p.phase ^= 1;
+  }
+  return p;
+}
+
+// The non-finite values that the check took out of the segment's partly seen
+// tiles, added to a row that sees them: 32 output columns.
+template <typename T>
+static __device__ __noinline__ void add_spoiled(const AttnParams& p, const AttnSegment& seg, const AttnSeq& s, uint32_t query,
+                                         uint32_t col0, float* o) {
+  const RowMask m = row_mask(p, s, query);
+  for (uint32_t il = seg.list0; il < seg.list1; ++il) {
+    const uint32_t e = p.lists[il];
+    if (entry_sees(e, 0) != kSeesSome && entry_sees(e, 1) != kSeesSome) continue;
+    for (uint32_t c = 0; c < kKeyTile; ++c) {
+      const uint32_t j = entry_tile(e) * kKeyTile + c;
+      if (j >= s.n_k) break;
+      if (!sees(p, m, j, p.doc_k ? p.doc_k[s.k0 + j] : 0)) continue;
+      const T* v = (const T*)p.v + (s.k0 + j) * p.ld_v + (uint64_t)seg.kvh * p.head_dim + col0;
+      for (uint32_t d = 0; d < 32 && col0 + d < p.head_dim; ++d) {
+        const float x = widen(v[d]);
+        if (!isfinite(x)) o[d] += x;
+      }
+    }
+  }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn encode_fn() {
+  static const EncodeTiledFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+                   q == cudaDriverEntryPointSuccess
+               ? (EncodeTiledFn)ptr
+               : nullptr;
+  }();
+  return fn;
+}
+
+// [rows][heads][head_dim] with 128-byte swizzled boxes of 64 columns, box_heads
+// heads and box_rows rows; columns behind the head read as zero.
+inline bool head_map(CUtensorMap* map, const void* base, uint32_t dtype, uint64_t rows, uint64_t heads, uint64_t head_dim,
+              uint64_t ld, uint32_t box_heads, uint32_t box_rows) {
+  const cuuint64_t dims[3] = {head_dim, heads, rows}, strides[2] = {head_dim * 2, ld * 2};
+  const cuuint32_t box[3] = {kSlabCols, box_heads, box_rows}, step[3] = {1, 1, 1};
+  return encode_fn()(map, dtype == SVL_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                     (void*)base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace svl

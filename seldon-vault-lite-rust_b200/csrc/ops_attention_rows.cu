@@ -1,0 +1,429 @@
+// ops_attention_rows.cu -- the FP16 / BF16 attention kernel of svl_attention_*
+// for few query rows (single tokens) over long key axes.
+//
+// Bound by reading K and V once.  A 128-row tensor-core tile would leave the
+// softmax of a handful of rows to a handful of threads, so the rows are the 16
+// rows of mma.sync m16n8k16 instead and eight warps take 16 keys each of every
+// 128-key tile: all lanes share the scores, and each warp keeps the running
+// maximum, sum and output of its own keys in registers, joined at the end.
+// K and V come by TMA through a ring of 16 KB slabs that one thread keeps full
+// across tiles and segments.  (A ninth warp for it would cut the registers of
+// the others from 255 to 168, the outputs of 32 rows or 256 columns out of them.)
+#include "ops_attention_mma.cuh"
+
+namespace svl {
+namespace {
+
+constexpr int kMmaWarps = 8, kThreads = kMmaWarps * 32;
+
+// MT tiles of 16 rows.
+template <int HDP, int MT>
+struct Smem {
+  static constexpr int kStages = 9, kRowBytes = HDP * 2 + 16;
+  alignas(1024) uint8_t ring[kStages * kSlabBytes];
+  float join[4][MT * 16][HDP];  // a join's outputs
+  uint8_t q[MT * 16 * kRowBytes];
+  float join_max[4][MT * 16], join_sum[4][MT * 16];
+  uint64_t full[kStages], empty[kStages];
+  uint32_t spoiled;
+};
+static_assert(sizeof(Smem<256, 1>) + 1024 <= kSmemLimit && sizeof(Smem<128, 2>) + 1024 <= kSmemLimit, "shared memory");
+
+SVL_DEV void ldmatrix(uint32_t* r, uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+SVL_DEV void ldmatrix_t(uint32_t* r, uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+SVL_DEV void mma(__half, float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+SVL_DEV void mma(__nv_bfloat16, float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The CTA's K and V slabs in the order in which they are used: of each segment's
+// key tiles, K's columns and then V's.
+template <int STAGES>
+struct Feeder {
+  RingPos pos;
+  uint32_t segment, entry, slab = 0, issued = 0;
+  int32_t row = 0, kvh = 0;
+  SVL_DEV Feeder(const AttnParams& p, uint32_t first, uint32_t end) : segment(first), entry(0) { enter(p, end, true); }
+  // Goes to the first key tile of this segment or the next that has one.
+  SVL_DEV void enter(const AttnParams& p, uint32_t end, bool fresh) {
+    for (; segment < end; ++segment, fresh = true) {
+      const AttnSegment& seg = p.segments[segment];
+      if (fresh) entry = seg.list0;
+      if (entry < seg.list1) {
+        kvh = (int32_t)seg.kvh;
+        row = (int32_t)(p.seqs[seg.seq].k0 + (uint64_t)entry_tile(p.lists[entry]) * kKeyTile);
+        return;
+      }
+    }
+  }
+  SVL_DEV void issue(const AttnParams& p, uint32_t end, uint8_t* ring, uint64_t* full, const CUtensorMap* k,
+                     const CUtensorMap* v, uint32_t slabs) {
+    mbar_arrive_expect_tx(&full[pos.stage], kSlabBytes);
+    tma_load_3d(ring + pos.stage * kSlabBytes, slab < slabs ? k : v, &full[pos.stage],
+                (int32_t)(slab < slabs ? slab : slab - slabs) * kSlabCols, kvh, row);
+    ++issued;
+    pos.next<STAGES>();
+    if (++slab == 2 * slabs) {
+      slab = 0;
+      ++entry;
+      enter(p, end, false);
+    }
+  }
+};
+
+// Zeroes the non-finite halves of an operand register.
+template <typename T>
+SVL_DEV bool clean(uint32_t& w) {
+  const uint32_t bad = non_finite(T(), w);
+  if (!bad) return false;
+  w &= ~((bad >> 15) * 0xffffu);
+  return true;
+}
+
+template <typename T, int HDP, int MT>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_rows_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap map_k,
+                          const __grid_constant__ CUtensorMap map_v) {
+  using Sm = Smem<HDP, MT>;
+  constexpr int kStages = Sm::kStages;
+  extern __shared__ uint8_t raw[];
+  Sm& sm = *(Sm*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slabs = (p.head_dim + kSlabCols - 1) / kSlabCols, steps = (p.head_dim + 15) / 16;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], kMmaWarps);
+    }
+    sm.spoiled = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  __syncthreads();
+  pdl_trigger();
+  const uint32_t seg0 = p.block_segments[blockIdx.x], seg1 = p.block_segments[blockIdx.x + 1];
+
+  const int g = lane >> 2, c2 = (lane & 3) * 2, mi = lane >> 3, mr = lane & 7;
+  const bool capped = p.cap > 0.0f, biased = p.slopes != nullptr;
+  const float scale2 = p.scale * kLog2e, cap2 = p.cap * kLog2e, cap_arg = capped ? 2.0f * scale2 / p.cap : 0.0f;
+  const uint32_t q_at = smem_u32(sm.q) + ((mi & 1) * 8 + mr) * Sm::kRowBytes + (mi >> 1) * 16;
+  // this warp's 16 keys of a slab: K by (8 keys, 8 columns) blocks, V by the same transposed
+  const uint32_t k_row = warp * 16 + (mi >> 1) * 8 + mr, v_row = warp * 16 + (mi & 1) * 8 + mr;
+  RingPos pos;
+  uint32_t used = 0;  // slabs that this warp is done with
+  bool dead = false;  // a wait ran out: no more waits, but every step is taken
+  Feeder<kStages> feeder(p, seg0, threadIdx.x == 0 ? seg1 : seg0);
+  const uint32_t feeds_to = threadIdx.x == 0 ? seg1 : seg0;
+  // Refills what everyone is done with.
+  auto feed = [&]() {
+    while (feeder.segment < feeds_to && mbar_test(&sm.empty[feeder.pos.stage], feeder.pos.phase ^ 1))
+      feeder.issue(p, feeds_to, sm.ring, sm.full, &map_k, &map_v, slabs);
+  };
+  auto wait = [&]() {
+    if (threadIdx.x == 0) {
+      feed();
+      // the slab that is next may still stand behind one that others use
+      while (!dead && feeder.issued <= used && feeder.segment < feeds_to) {
+        if (!mbar_wait(&sm.empty[feeder.pos.stage], feeder.pos.phase ^ 1, p.err)) dead = true;
+        else feeder.issue(p, feeds_to, sm.ring, sm.full, &map_k, &map_v, slabs);
+      }
+    }
+    __syncwarp();
+    if (!dead && !mbar_wait(&sm.full[pos.stage], pos.phase, p.err)) dead = true;
+    __syncwarp();
+  };
+  auto done = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.empty[pos.stage]);
+    pos.next<kStages>();
+    ++used;
+  };
+
+  for (uint32_t is = seg0; is < seg1; ++is) {
+    const AttnSegment seg = p.segments[is];
+    const AttnSeq s = p.seqs[seg.seq];
+    __syncthreads();  // the last segment's rows and flags are read
+    for (int i = threadIdx.x; i < MT * 16 * (HDP / 8); i += kMmaWarps * 32) {
+      const int r = i / (HDP / 8), d = i % (HDP / 8) * 8;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      const uint32_t row = seg.row0 + r;
+      if (r < (int)seg.rows && d < (int)p.head_dim)
+        w = *(const uint4*)((const T*)p.q + (s.q0 + row / p.group) * p.ld_q +
+                            (uint64_t)(seg.kvh * p.group + row % p.group) * p.head_dim + d);
+      *(uint4*)(sm.q + r * Sm::kRowBytes + d * 2) = w;
+    }
+    if (threadIdx.x == 0) {
+      sm.spoiled = 0;
+      feed();
+    }
+    // this thread's rows: g and g + 8 of each row tile
+    RowMask mask[MT][2];
+    float slope2[MT][2], m[MT][2], l[MT][2], o[MT][HDP / 8][4];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t row = seg.row0 + min((uint32_t)(t * 16 + u * 8 + g), seg.rows - 1);
+        mask[t][u] = row_mask(p, s, row / p.group);
+        slope2[t][u] = biased ? p.slopes[seg.kvh * p.group + row % p.group] * kLog2e : 0.0f;
+        m[t][u] = -INFINITY;
+        l[t][u] = 0.0f;
+      }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int d = 0; d < HDP / 8; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[t][d][e] = 0.0f;
+    __syncthreads();
+
+    uint32_t next = seg.list0 < seg.list1 ? p.lists[seg.list0] : 0;
+#pragma unroll 1
+    for (uint32_t il = seg.list0; il < seg.list1; ++il) {
+      const uint32_t entry = next;
+      if (il + 1 < seg.list1) next = p.lists[il + 1];
+      const uint32_t j0 = entry_tile(entry) * kKeyTile + warp * 16;
+      const bool some = entry_sees(entry, 0) == kSeesSome;
+      // scores of 16 keys: tiles of 8
+      float sc[MT][2][4] = {};
+#pragma unroll
+      for (int c = 0; c < HDP / kSlabCols; ++c) {
+        if (c >= slabs) break;
+        wait();
+        const uint32_t slab = smem_u32(sm.ring) + pos.stage * kSlabBytes + k_row * 128;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (c * 4 + k >= steps) break;
+          uint32_t b[4], a[4];
+          ldmatrix(b, slab + ((2 * k + (mi & 1)) ^ mr) * 16);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            ldmatrix(a, q_at + t * 16 * Sm::kRowBytes + (c * 4 + k) * 32);
+            mma(T(), sc[t][0], a, b[0], b[1]);
+            mma(T(), sc[t][1], a, b[2], b[3]);
+          }
+        }
+        done();
+      }
+      uint32_t pa[MT][4];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int u = e >> 1;
+            const uint32_t j = j0 + n * 8 + c2 + (e & 1);
+            float x = sc[t][n][e];
+            // cap tanh(y) = cap - 2 cap / (1 + e^2y), in log2 units
+            x = capped ? cap2 - __fdividef(2.0f * cap2, 1.0f + ex2_approx(x * cap_arg)) : x * scale2;
+            if (biased) x = fmaf(-slope2[t][u], fabsf((float)(mask[t][u].place - (int64_t)j)), x);
+            if (some && !sees(p, mask[t][u], j, p.doc_k && j < s.n_k ? __ldg(p.doc_k + s.k0 + j) : 0)) x = -INFINITY;
+            sc[t][n][e] = x;
+          }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float top = fmaxf(fmaxf(sc[t][0][2 * u], sc[t][0][2 * u + 1]), fmaxf(sc[t][1][2 * u], sc[t][1][2 * u + 1]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          float factor = 1.0f;
+          if (top > m[t][u] + kBehind || (m[t][u] == -INFINITY && top > -INFINITY)) {
+            factor = m[t][u] == -INFINITY ? 0.0f : ex2_approx(m[t][u] - top);
+            m[t][u] = top;
+          }
+          if (__any_sync(0xffffffffu, factor != 1.0f)) {
+            l[t][u] *= factor;
+#pragma unroll
+            for (int d = 0; d < HDP / 8; ++d) {
+              o[t][d][2 * u] *= factor;
+              o[t][d][2 * u + 1] *= factor;
+            }
+          }
+          const float base = m[t][u] == -INFINITY ? 0.0f : m[t][u];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const float x = ex2_approx(sc[t][n][2 * u] - base), y = ex2_approx(sc[t][n][2 * u + 1] - base);
+            l[t][u] += x + y;
+            pa[t][2 * n + u] = pack2(T(), x, y);
+          }
+        }
+      }
+      bool found = false;
+#pragma unroll
+      for (int c = 0; c < HDP / kSlabCols; ++c) {
+        if (c >= slabs) break;
+        wait();
+        const uint32_t slab = smem_u32(sm.ring) + pos.stage * kSlabBytes + v_row * 128;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (c * 4 + k >= steps) break;
+          uint32_t b[4];
+          ldmatrix_t(b, slab + ((2 * k + (mi >> 1)) ^ mr) * 16);
+          if (some) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) found |= clean<T>(b[i]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            mma(T(), o[t][(c * 4 + k) * 2], pa[t], b[0], b[1]);
+            mma(T(), o[t][(c * 4 + k) * 2 + 1], pa[t], b[2], b[3]);
+          }
+        }
+        done();
+      }
+      if (some && __any_sync(0xffffffffu, found) && lane == 0) atomicOr(&sm.spoiled, 1u);
+    }
+    // A row's sum lies over its four lanes; then the warps join in halves: the
+    // upper half hands maximum, sum and output over, the lower half adds them.
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        l[t][u] += __shfl_xor_sync(0xffffffffu, l[t][u], 1);
+        l[t][u] += __shfl_xor_sync(0xffffffffu, l[t][u], 2);
+      }
+#pragma unroll 1
+    for (int half = kMmaWarps / 2; half >= 1; half /= 2) {
+      if (warp >= half && warp < 2 * half) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int r = t * 16 + u * 8 + g;
+            if (c2 == 0) {
+              sm.join_max[warp - half][r] = m[t][u];
+              sm.join_sum[warp - half][r] = l[t][u];
+            }
+#pragma unroll
+            for (int d = 0; d < HDP / 8; ++d)
+              *(float2*)&sm.join[warp - half][r][d * 8 + c2] = make_float2(o[t][d][2 * u], o[t][d][2 * u + 1]);
+          }
+      }
+      __syncthreads();
+      if (warp < half) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int r = t * 16 + u * 8 + g;
+            const float other = sm.join_max[warp][r], top = fmaxf(m[t][u], other);
+            const float mine = m[t][u] == -INFINITY ? 0.0f : ex2_approx(m[t][u] - top);
+            const float theirs = other == -INFINITY ? 0.0f : ex2_approx(other - top);
+            // a sum that is NaN with a maximum of -inf (every score NaN) stays
+            const float their_sum = sm.join_sum[warp][r];
+            l[t][u] = (l[t][u] != l[t][u] || their_sum != their_sum) ? NAN : l[t][u] * mine + their_sum * theirs;
+            m[t][u] = top;
+#pragma unroll
+            for (int d = 0; d < HDP / 8; ++d) {
+              const float2 w = *(const float2*)&sm.join[warp][r][d * 8 + c2];
+              // nothing is taken from a side without weight: what it holds is 0
+              if (mine != 1.0f) o[t][d][2 * u] *= mine, o[t][d][2 * u + 1] *= mine;
+              o[t][d][2 * u] = fmaf(w.x, theirs, o[t][d][2 * u]);
+              o[t][d][2 * u + 1] = fmaf(w.y, theirs, o[t][d][2 * u + 1]);
+            }
+          }
+      }
+      __syncthreads();
+    }
+    if (warp != 0) continue;
+    const bool spoiled = sm.spoiled != 0;
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t in_seg = t * 16 + u * 8 + g;
+        if (in_seg >= seg.rows) continue;
+        const uint32_t row = seg.row0 + in_seg, query = row / p.group, head = seg.kvh * p.group + row % p.group;
+        const uint64_t token = s.q0 + query, part = (uint64_t)(seg.slot < 0 ? 0 : seg.slot) * p.slot_rows + in_seg;
+        const bool empty = m[t][u] == -INFINITY && l[t][u] == 0.0f;
+        const float inv = empty ? 0.0f : 1.0f / l[t][u];
+        const float lse = empty ? -INFINITY : kLn2 * ((m[t][u] == -INFINITY ? 0.0f : m[t][u]) + log2f(l[t][u]));
+        if (c2 == 0) {
+          if (seg.slot >= 0) p.part_lse[part] = lse;
+          else if (p.lse) p.lse[token * p.q_heads + head] = lse;
+        }
+#pragma unroll
+        for (int d = 0; d < HDP / 8; ++d) {
+          const uint32_t col = d * 8 + c2;
+          if (col >= p.head_dim) break;
+          float2 w = make_float2(empty ? 0.0f : o[t][d][2 * u] * inv, empty ? 0.0f : o[t][d][2 * u + 1] * inv);
+          if (spoiled) {
+            float extra[32];
+            for (int i = 0; i < 32; ++i) extra[i] = 0.0f;
+            add_spoiled<T>(p, seg, s, query, col, extra);
+            w.x += extra[0];
+            w.y += extra[1];
+          }
+          if (seg.slot >= 0) *(float2*)(p.part_o + part * p.head_dim + col) = w;
+          else *(uint32_t*)((T*)p.out + token * p.ld_out + (uint64_t)head * p.head_dim + col) = pack2(T(), w.x, w.y);
+        }
+      }
+  }
+  if (threadIdx.x == 0 && dead) {
+    // copies in flight land before the CTA leaves
+    RingPos back;
+    for (uint32_t i = 0; i < feeder.issued; ++i) {
+      if (i + kStages >= feeder.issued) mbar_wait(&sm.full[back.stage], back.phase, p.err);
+      back.next<kStages>();
+    }
+  }
+}
+
+template <typename T, int HDP, int MT>
+cudaError_t launch(const AttnParams& p, uint32_t dtype, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  const int smem = (int)sizeof(Smem<HDP, MT>) + 1024;
+  const cudaError_t e = smem_opt_in(attention_rows_kernel<T, HDP, MT>, smem, &done);
+  if (e != cudaSuccess) return e;
+  CUtensorMap k, v;
+  // without keys there is nothing to load: any valid map will do
+  const bool keys = p.total_k > 0;
+  if (!encode_fn() ||
+      !head_map(&k, keys ? p.k : p.q, dtype, keys ? p.total_k : 1, keys ? p.kv_heads : 1, p.head_dim, keys ? p.ld_k : p.ld_q,
+                1, kKeyTile) ||
+      !head_map(&v, keys ? p.v : p.q, dtype, keys ? p.total_k : 1, keys ? p.kv_heads : 1, p.head_dim, keys ? p.ld_v : p.ld_q,
+                1, kKeyTile))
+    return cudaErrorInvalidValue;
+  attention_rows_kernel<T, HDP, MT><<<p.blocks, kThreads, smem, st>>>(p, k, v);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch(const AttnParams& p, uint32_t dtype, cudaStream_t st) {
+  const bool two = p.slot_rows > 16;
+  if (p.head_dim <= 64) return two ? launch<T, 64, 2>(p, dtype, st) : launch<T, 64, 1>(p, dtype, st);
+  if (p.head_dim <= 128) return two ? launch<T, 128, 2>(p, dtype, st) : launch<T, 128, 1>(p, dtype, st);
+  return launch<T, 256, 1>(p, dtype, st);
+}
+
+}  // namespace
+
+uint32_t attention_rows_takes(uint32_t head_dim, uint64_t rows) {
+  return rows <= 16 ? 16 : rows <= 32 && head_dim <= 128 ? 32 : 0;
+}
+
+cudaError_t attention_rows_launch(const AttnParams& p, uint32_t dtype, cudaStream_t st) {
+  return dtype == SVL_DTYPE_F16 ? launch<__half>(p, dtype, st) : launch<__nv_bfloat16>(p, dtype, st);
+}
+
+}  // namespace svl

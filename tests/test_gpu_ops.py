@@ -516,6 +516,23 @@ def test_attention_hidden_values(dtype, spoil, kwargs):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("spoil", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("hq,hk,hd", [(4, 2, 64), (8, 1, 128), (2, 2, 256), (3, 1, 72)])
+def test_attention_few_rows_hidden_values(dtype, spoil, hq, hk, hd):
+    run_attention(dtype, hq, hk, hd, [(2, 500), (1, 131), (3, 64), (4, 1290)], spoil=spoil, docs=runs_of(90, 1), window=40)
+    run_attention(dtype, hq, hk, hd, [(2, 500), (1, 131), (3, 64), (1, 129)], spoil=spoil, causal=True, window=3,
+                  docs=runs_of(10 ** 6, 0))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hq,hk,hd", HEADS + [(2, 1, 512), (1, 1, 8), (32, 1, 64), (16, 1, 256), (12, 1, 128)])
+@pytest.mark.parametrize("kwargs", [{}, dict(cap=4.0, slopes=True), dict(causal=True, window=200, docs=runs_of(300, 1)),
+                                    dict(docs=shuffled, prefix=[3, 0, 130])], ids=lambda d: ",".join(d) or "plain")
+def test_attention_few_rows(dtype, hq, hk, hd, kwargs):
+    run_attention(dtype, hq, hk, hd, [(1, 700), (2, 129), (1, 1)], **kwargs)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_attention_value_seen_by_some(dtype, hd, bad):
@@ -535,6 +552,19 @@ def test_attention_value_seen_by_some(dtype, hd, bad):
         p = torch.arange(n, device="cuda")
         sees = (p >= at) if causal else ((p - at).abs() <= window) if window else torch.ones_like(p, dtype=torch.bool)
         want = torch.zeros(n, hd, dtype=torch.bool, device="cuda")
+        # the last eight rows alone: the kernel for few rows
+        few = AttentionPlan(1, 1, hd, [0, 8], [0, n], dtype=dtype, causal=causal, window=window and 97)
+        part = torch.empty(8, hd, device="cuda", dtype=t)
+        ws = torch.empty(few.workspace_bytes, dtype=torch.uint8, device="cuda")
+        few.run_device(q[-8:].data_ptr(), 3 * hd, k.data_ptr(), 3 * hd, v.data_ptr(), 3 * hd, part.data_ptr(), hd,
+                       workspace=ws.data_ptr(), workspace_bytes=few.workspace_bytes, stream=stream())
+        few.check()
+        near = (p[-8:] - at <= 97) if window else torch.ones_like(p[-8:], dtype=torch.bool)
+        seen = torch.zeros(8, hd, dtype=torch.bool, device="cuda")
+        seen[near, col] = True
+        assert torch.equal(~torch.isfinite(part.float()), seen)
+        if not math.isnan(bad):
+            assert (part[near, col].float() == bad).all()
         want[sees, col] = True
         assert torch.equal(~torch.isfinite(out.float()), want)
         if not math.isnan(bad):
