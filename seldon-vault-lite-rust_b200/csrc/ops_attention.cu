@@ -5,7 +5,7 @@
 #include <climits>
 #include <vector>
 
-#include "ops_attention.cuh"
+#include "ops_attention_mma.cuh"
 
 namespace svl {
 namespace {
@@ -195,43 +195,65 @@ __global__ void __launch_bounds__(kGenThreads) attention_general_kernel(const __
 
 // ---------------------------------------------------------------- the join --
 //
-// out = sum_s e^(lse_s - lse) out_s with lse = log sum_s e^lse_s: one warp a row.
+// out = sum_s e^(lse_s - lse) out_s with lse = log sum_s e^lse_s: one block a
+// row.  Its weights go to shared memory a batch at a time, and the threads take
+// the columns, so that the loads of a batch do not wait for one another.
+constexpr int kJoinThreads = 128, kJoinBatch = 128;
 template <typename T>
-__global__ void attention_join_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttnParams p) {
+  __shared__ float weight[kJoinBatch], all[2][kJoinThreads / 32];
   pdl_wait();  // the parts; launch_pdl's rule
   const AttnJoin j = p.joins[blockIdx.x];
+  const uint32_t r = blockIdx.y;
+  if (r >= j.rows) return;
   const AttnSeq s = p.seqs[j.seq];
-  const int lane = threadIdx.x & 31;
-  for (uint32_t r = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5); r < j.rows; r += gridDim.y * (blockDim.x >> 5)) {
-    const uint32_t row = j.row0 + r;
-    const uint64_t token = s.q0 + row / p.group;
-    const uint32_t head = j.kvh * p.group + row % p.group;
-    float m = -INFINITY;
-    bool nan = false;
-    for (uint32_t c = lane; c < j.slots; c += 32) {
-      const float l = p.part_lse[(uint64_t)(j.slot0 + c) * p.slot_rows + r];
-      m = fmaxf(m, l);
-      nan |= l != l;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t row = j.row0 + r, head = j.kvh * p.group + row % p.group;
+  const uint64_t token = s.q0 + row / p.group;
+  const float* lse = p.part_lse + (uint64_t)j.slot0 * p.slot_rows + r;
+  const float* part = p.part_o + ((uint64_t)j.slot0 * p.slot_rows + r) * p.head_dim;
+  const uint64_t lse_step = p.slot_rows, part_step = (uint64_t)p.slot_rows * p.head_dim;
+  float m = -INFINITY;
+  for (uint32_t c = tid; c < j.slots; c += kJoinThreads) m = fmaxf(m, lse[c * lse_step]);
+  m = warp_max(m);
+  if (lane == 0) all[0][warp] = m;
+  __syncthreads();
+  for (int w = 0; w < kJoinThreads / 32; ++w) m = fmaxf(m, all[0][w]);
+  const float base = m == -INFINITY ? 0.0f : m;
+  float sum = 0.0f, o[kAttnMaxHead / kJoinThreads] = {};
+  for (uint32_t c0 = 0; c0 < j.slots; c0 += kJoinBatch) {
+    const uint32_t n = min((uint32_t)kJoinBatch, j.slots - c0);
+    __syncthreads();
+    if (tid < (int)n) {
+      const float w = expf(lse[(c0 + tid) * lse_step] - base);  // NaN where a part's rows are
+      weight[tid] = w;
+      sum += w;
     }
-    m = warp_max(m);
-    nan = __any_sync(0xffffffffu, nan);
-    const float base = m == -INFINITY ? 0.0f : m;
-    float sum = 0.0f;
-    for (uint32_t c = lane; c < j.slots; c += 32)
-      sum += expf(p.part_lse[(uint64_t)(j.slot0 + c) * p.slot_rows + r] - base);
-    sum = warp_sum(sum);
-    const float inv = sum > 0.0f || nan ? 1.0f / sum : 0.0f;
-    for (uint32_t d = lane; d < p.head_dim; d += 32) {
-      float o = 0.0f;
-      for (uint32_t c = 0; c < j.slots; ++c) {
-        const uint64_t part = (uint64_t)(j.slot0 + c) * p.slot_rows + r;
-        const float l = p.part_lse[part];
-        if (l != -INFINITY) o = fmaf(expf(l - base), p.part_o[part * p.head_dim + d], o);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kAttnMaxHead / kJoinThreads; ++u) {
+      const uint32_t d = u * kJoinThreads + tid;
+      if (d >= p.head_dim) break;
+#pragma unroll 8
+      for (uint32_t c = 0; c < n; ++c) {
+        const float x = part[(c0 + c) * part_step + d];
+        if (weight[c] != 0.0f) o[u] = fmaf(weight[c], x, o[u]);
       }
-      ((T*)p.out)[token * p.ld_out + (uint64_t)head * p.head_dim + d] = narrow<T>(o * inv);
     }
-    if (lane == 0 && p.lse) p.lse[token * p.q_heads + head] = sum > 0.0f || nan ? base + logf(sum) : -INFINITY;
   }
+  sum = warp_sum(sum);
+  if (lane == 0) all[1][warp] = sum;
+  __syncthreads();
+  sum = 0.0f;
+  for (int w = 0; w < kJoinThreads / 32; ++w) sum += all[1][w];
+  const bool empty = sum == 0.0f;
+  const float inv = empty ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int u = 0; u < kAttnMaxHead / kJoinThreads; ++u) {
+    const uint32_t d = u * kJoinThreads + tid;
+    if (d < p.head_dim) ((T*)p.out)[token * p.ld_out + (uint64_t)head * p.head_dim + d] = narrow<T>(o[u] * inv);
+  }
+  if (tid == 0 && p.lse) p.lse[token * p.q_heads + head] = empty ? -INFINITY : base + logf(sum);
 }
 
 }  // namespace
@@ -475,7 +497,7 @@ cudaError_t launch_general(const svl::AttnParams& p, cudaStream_t st) {
 
 template <typename T>
 cudaError_t launch_join(const svl::AttnParams& p, uint32_t rows, cudaStream_t st) {
-  return launch_pdl(svl::attention_join_kernel<T>, dim3(p.n_joins, (rows + 7) / 8), dim3(256), 0, st, p);
+  return launch_pdl(svl::attention_join_kernel<T>, dim3(p.n_joins, rows), dim3(svl::kJoinThreads), 0, st, p);
 }
 
 // Blocks of the general kernel an SM takes (its shared memory allows two at
@@ -587,6 +609,12 @@ int svl_attention_plan_create(int device, const svl_attention_config* config, co
     p.total_k = n_k;
     p.scale = c.scale;
     p.cap = c.cap;
+    if (c.cap > 0) {
+      const double k = (double)c.scale / c.cap;
+      double power = (double)c.cap * 1.4426950408889634 * k;
+      for (int i = 0; i < 5; ++i, power *= k * k) p.cap_odd[i] = (float)(power * svl::kTanhOdd[i]);
+      p.cap_limit = (float)std::min(0.5 / k, 3.0e38);
+    }
     p.causal = (int32_t)c.causal;
     p.window = c.window;
     plan->max_join_rows = s.max_join_rows;

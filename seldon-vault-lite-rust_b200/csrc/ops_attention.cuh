@@ -53,6 +53,7 @@ struct AttnParams {
   uint32_t q_heads, kv_heads, group, head_dim;
   uint64_t total_q, total_k;
   float scale, cap;
+  float cap_odd[5], cap_limit;  // capped_small() below
   int32_t causal, window;
   // one call's operands
   const void *q, *k, *v;

@@ -13,6 +13,23 @@ constexpr int kSmemLimit = 232448;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kBehind = 8.0f;  // a maximum follows once it is 2^8 behind (log2 units)
 
+// cap tanh(scale s / cap) of a raw score s in log2 units.  tanh y = y P(y^2) with
+// P of degree 4 fitted to tanh(y) / y for |y| <= 1/2 (relative error 1.3e-8, below
+// FP32's half step): five multiply-adds on the FMA pipe, with the cap and scale
+// in the coefficients.  The general form costs two of the 16 special functions a
+// cycle that the softmax itself needs; a warp takes it when a score of its tile
+// lies behind cap_limit = cap / (2 scale).
+constexpr double kTanhOdd[5] = {0.9999999873738349, -0.33333075792040845, 0.133249069544671, -0.052994230404600086,
+                                0.017151297500408665};
+SVL_DEV float capped_small(const AttnParams& p, float s) {
+  const float z = s * s;
+  return s * fmaf(z, fmaf(z, fmaf(z, fmaf(z, p.cap_odd[4], p.cap_odd[3]), p.cap_odd[2]), p.cap_odd[1]), p.cap_odd[0]);
+}
+// cap - 2 cap / (1 + e^2y); arg = 2 log2(e) scale / cap, cap2 = cap log2(e)
+SVL_DEV float capped_any(float s, float arg, float cap2) {
+  return cap2 - __fdividef(2.0f * cap2, 1.0f + ex2_approx(s * arg));
+}
+
 SVL_DEV uint32_t pack2(__half, float lo, float hi) { return pack_half2(lo, hi); }
 SVL_DEV uint32_t pack2(__nv_bfloat16, float lo, float hi) {
   uint32_t r;

@@ -3,9 +3,10 @@
 //
 // Bound by reading K and V once.  A 128-row tensor-core tile would leave the
 // softmax of a handful of rows to a handful of threads, so the rows are the 16
-// rows of mma.sync m16n8k16 instead and eight warps take 16 keys each of every
-// 128-key tile: all lanes share the scores, and each warp keeps the running
-// maximum, sum and output of its own keys in registers, joined at the end.
+// rows of mma.sync m16n8k16 instead: all lanes share the scores.  Two teams of
+// four warps take every other 128-key tile, 32 keys a warp, and each warp keeps
+// the running maximum, sum and output of its own keys in registers, joined at the
+// end.
 // K and V come by TMA through a ring of 16 KB slabs that one thread keeps full
 // across tiles and segments.  (A ninth warp for it would cut the registers of
 // the others from 255 to 168, the outputs of 32 rows or 256 columns out of them.)
@@ -14,7 +15,7 @@
 namespace svl {
 namespace {
 
-constexpr int kMmaWarps = 8, kThreads = kMmaWarps * 32;
+constexpr int kMmaWarps = 8, kThreads = kMmaWarps * 32, kTeam = kMmaWarps / 2, kKeys = 2;  // 16s of keys a warp
 
 // MT tiles of 16 rows.
 template <int HDP, int MT>
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sm.full[i], 1);
-      mbar_init(&sm.empty[i], kMmaWarps);
+      mbar_init(&sm.empty[i], kTeam);
     }
     sm.spoiled = 0;
     fence_barrier_init();
@@ -126,26 +127,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool capped = p.cap > 0.0f, biased = p.slopes != nullptr;
   const float scale2 = p.scale * kLog2e, cap2 = p.cap * kLog2e, cap_arg = capped ? 2.0f * scale2 / p.cap : 0.0f;
   const uint32_t q_at = smem_u32(sm.q) + ((mi & 1) * 8 + mr) * Sm::kRowBytes + (mi >> 1) * 16;
-  // this warp's 16 keys of a slab: K by (8 keys, 8 columns) blocks, V by the same transposed
-  const uint32_t k_row = warp * 16 + (mi >> 1) * 8 + mr, v_row = warp * 16 + (mi & 1) * 8 + mr;
+  // this warp's keys of a slab: K by (8 keys, 8 columns) blocks, V by the same transposed
+  const int team = warp / kTeam, key0 = warp % kTeam * 16 * kKeys;
+  const uint32_t k_row = key0 + (mi >> 1) * 8 + mr, v_row = key0 + (mi & 1) * 8 + mr;
   RingPos pos;
-  uint32_t used = 0;  // slabs that this warp is done with
-  bool dead = false;  // a wait ran out: no more waits, but every step is taken
-  Feeder<kStages> feeder(p, seg0, threadIdx.x == 0 ? seg1 : seg0);
+  uint32_t at = 0;     // the CTA's slabs before this segment, then the slab that this warp is at
+  bool dead = false;   // a wait ran out: no more waits, but every step is taken
   const uint32_t feeds_to = threadIdx.x == 0 ? seg1 : seg0;
-  // Refills what everyone is done with.
+  Feeder<kStages> feeder(p, seg0, feeds_to);
+  // Refills what its team is done with.
   auto feed = [&]() {
     while (feeder.segment < feeds_to && mbar_test(&sm.empty[feeder.pos.stage], feeder.pos.phase ^ 1))
       feeder.issue(p, feeds_to, sm.ring, sm.full, &map_k, &map_v, slabs);
   };
+  // The first `n` slabs, if need be behind slabs that are still in use.
+  auto feed_up_to = [&](uint32_t n) {
+    while (!dead && feeder.issued < n && feeder.segment < feeds_to) {
+      if (!mbar_wait(&sm.empty[feeder.pos.stage], feeder.pos.phase ^ 1, p.err)) dead = true;
+      else feeder.issue(p, feeds_to, sm.ring, sm.full, &map_k, &map_v, slabs);
+    }
+  };
   auto wait = [&]() {
     if (threadIdx.x == 0) {
       feed();
-      // the slab that is next may still stand behind one that others use
-      while (!dead && feeder.issued <= used && feeder.segment < feeds_to) {
-        if (!mbar_wait(&sm.empty[feeder.pos.stage], feeder.pos.phase ^ 1, p.err)) dead = true;
-        else feeder.issue(p, feeds_to, sm.ring, sm.full, &map_k, &map_v, slabs);
-      }
+      feed_up_to(at + 1);
     }
     __syncwarp();
     if (!dead && !mbar_wait(&sm.full[pos.stage], pos.phase, p.err)) dead = true;
@@ -155,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.empty[pos.stage]);
     pos.next<kStages>();
-    ++used;
+    ++at;
   };
 
   for (uint32_t is = seg0; is < seg1; ++is) {
@@ -196,15 +201,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < 4; ++e) o[t][d][e] = 0.0f;
     __syncthreads();
 
-    uint32_t next = seg.list0 < seg.list1 ? p.lists[seg.list0] : 0;
+    const uint32_t slabs0 = at;
+    uint32_t next = seg.list0 + team < seg.list1 ? p.lists[seg.list0 + team] : 0;
 #pragma unroll 1
-    for (uint32_t il = seg.list0; il < seg.list1; ++il) {
+    for (uint32_t il = seg.list0 + team; il < seg.list1; il += 2) {
       const uint32_t entry = next;
-      if (il + 1 < seg.list1) next = p.lists[il + 1];
-      const uint32_t j0 = entry_tile(entry) * kKeyTile + warp * 16;
+      if (il + 2 < seg.list1) next = p.lists[il + 2];
+      at = slabs0 + (il - seg.list0) * 2 * slabs;
+      pos.stage = at % kStages;
+      pos.phase = at / kStages & 1;
+      const uint32_t j0 = entry_tile(entry) * kKeyTile + key0;
       const bool some = entry_sees(entry, 0) == kSeesSome;
-      // scores of 16 keys: tiles of 8
-      float sc[MT][2][4] = {};
+      // scores: tiles of 8 keys
+      float sc[MT][2 * kKeys][4] = {};
 #pragma unroll
       for (int c = 0; c < HDP / kSlabCols; ++c) {
         if (c >= slabs) break;
@@ -213,36 +222,72 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (c * 4 + k >= steps) break;
-          uint32_t b[4], a[4];
-          ldmatrix(b, slab + ((2 * k + (mi & 1)) ^ mr) * 16);
+          uint32_t b[kKeys][4];
+#pragma unroll
+          for (int n = 0; n < kKeys; ++n) ldmatrix(b[n], slab + n * 2048 + ((2 * k + (mi & 1)) ^ mr) * 16);
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
+            uint32_t a[4];
             ldmatrix(a, q_at + t * 16 * Sm::kRowBytes + (c * 4 + k) * 32);
-            mma(T(), sc[t][0], a, b[0], b[1]);
-            mma(T(), sc[t][1], a, b[2], b[3]);
+#pragma unroll
+            for (int n = 0; n < kKeys; ++n) {
+              mma(T(), sc[t][2 * n], a, b[n][0], b[n][1]);
+              mma(T(), sc[t][2 * n + 1], a, b[n][2], b[n][3]);
+            }
           }
         }
         done();
       }
-      uint32_t pa[MT][4];
+      uint32_t pa[MT][kKeys][4];
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
+        if (capped) {
+          float most = 0.0f;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < 2 * kKeys; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int u = e >> 1;
-            const uint32_t j = j0 + n * 8 + c2 + (e & 1);
-            float x = sc[t][n][e];
-            // cap tanh(y) = cap - 2 cap / (1 + e^2y), in log2 units
-            x = capped ? cap2 - __fdividef(2.0f * cap2, 1.0f + ex2_approx(x * cap_arg)) : x * scale2;
-            if (biased) x = fmaf(-slope2[t][u], fabsf((float)(mask[t][u].place - (int64_t)j)), x);
-            if (some && !sees(p, mask[t][u], j, p.doc_k && j < s.n_k ? __ldg(p.doc_k + s.k0 + j) : 0)) x = -INFINITY;
-            sc[t][n][e] = x;
+            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(sc[t][n][e]));
+          if (__any_sync(0xffffffffu, most > p.cap_limit)) {
+#pragma unroll
+            for (int n = 0; n < 2 * kKeys; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[t][n][e] = capped_any(sc[t][n][e], cap_arg, cap2);
+          } else {
+#pragma unroll
+            for (int n = 0; n < 2 * kKeys; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[t][n][e] = capped_small(p, sc[t][n][e]);
           }
+        } else {
+#pragma unroll
+          for (int n = 0; n < 2 * kKeys; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[t][n][e] *= scale2;
+        }
+        if (biased) {
+#pragma unroll
+          for (int n = 0; n < 2 * kKeys; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int64_t gap = mask[t][e >> 1].place - (int64_t)(j0 + n * 8 + c2 + (e & 1));
+              sc[t][n][e] = fmaf(-slope2[t][e >> 1], fabsf((float)gap), sc[t][n][e]);
+            }
+        }
+        if (some) {
+#pragma unroll
+          for (int n = 0; n < 2 * kKeys; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t j = j0 + n * 8 + c2 + (e & 1);
+              if (!sees(p, mask[t][e >> 1], j, p.doc_k && j < s.n_k ? __ldg(p.doc_k + s.k0 + j) : 0))
+                sc[t][n][e] = -INFINITY;
+            }
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          float top = fmaxf(fmaxf(sc[t][0][2 * u], sc[t][0][2 * u + 1]), fmaxf(sc[t][1][2 * u], sc[t][1][2 * u + 1]));
+          float top = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < 2 * kKeys; ++n) top = fmax3(top, sc[t][n][2 * u], sc[t][n][2 * u + 1]);
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           float factor = 1.0f;
@@ -260,10 +305,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const float base = m[t][u] == -INFINITY ? 0.0f : m[t][u];
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
+          for (int n = 0; n < 2 * kKeys; ++n) {
             const float x = ex2_approx(sc[t][n][2 * u] - base), y = ex2_approx(sc[t][n][2 * u + 1] - base);
             l[t][u] += x + y;
-            pa[t][2 * n + u] = pack2(T(), x, y);
+            pa[t][n >> 1][2 * (n & 1) + u] = pack2(T(), x, y);
           }
         }
       }
@@ -276,23 +321,32 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (c * 4 + k >= steps) break;
-          uint32_t b[4];
-          ldmatrix_t(b, slab + ((2 * k + (mi >> 1)) ^ mr) * 16);
-          if (some) {
+          uint32_t b[kKeys][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) found |= clean<T>(b[i]);
+          for (int n = 0; n < kKeys; ++n) {
+            ldmatrix_t(b[n], slab + n * 2048 + ((2 * k + (mi >> 1)) ^ mr) * 16);
+            if (some) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) found |= clean<T>(b[n][i]);
+            }
           }
           __syncwarp();
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            mma(T(), o[t][(c * 4 + k) * 2], pa[t], b[0], b[1]);
-            mma(T(), o[t][(c * 4 + k) * 2 + 1], pa[t], b[2], b[3]);
-          }
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int n = 0; n < kKeys; ++n) {
+              mma(T(), o[t][(c * 4 + k) * 2], pa[t][n], b[n][0], b[n][1]);
+              mma(T(), o[t][(c * 4 + k) * 2 + 1], pa[t][n], b[n][2], b[n][3]);
+            }
         }
         done();
       }
       if (some && __any_sync(0xffffffffu, found) && lane == 0) atomicOr(&sm.spoiled, 1u);
     }
+    // the other team's last tile, before this warp waits for it
+    at = slabs0 + (seg.list1 - seg.list0) * 2 * slabs;
+    if (threadIdx.x == 0) feed_up_to(at);
+    __syncwarp();
     // A row's sum lies over its four lanes; then the warps join in halves: the
     // upper half hands maximum, sum and output over, the lower half adds them.
 #pragma unroll

@@ -417,10 +417,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto x = [&](int c) { return __uint_as_float(w[c]); };
         const int64_t j0 = (int64_t)entry_tile(e) * kKeyTile + half * kCols;
         if (capped) {
-          // cap tanh(y) = cap - 2 cap / (1 + e^2y), in log2 units
+          float most = 0.0f;
 #pragma unroll
-          for (int c = 0; c < kCols; ++c)
-            w[c] = __float_as_uint(cap2 - __fdividef(2.0f * cap2, 1.0f + ex2_approx(x(c) * cap_arg)));
+          for (int c = 0; c < kCols; c += 2) most = fmax3(most, fabsf(x(c)), fabsf(x(c + 1)));
+          if (__any_sync(0xffffffffu, most > p.cap_limit)) {
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) w[c] = __float_as_uint(capped_any(x(c), cap_arg, cap2));
+          } else {
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) w[c] = __float_as_uint(capped_small(p, x(c)));
+          }
         } else if (biased) {
 #pragma unroll
           for (int c = 0; c < kCols; ++c) w[c] = __float_as_uint(x(c) * scale2);
