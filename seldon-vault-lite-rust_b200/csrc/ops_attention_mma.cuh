@@ -25,6 +25,60 @@ SVL_DEV float capped_small(const AttnParams& p, float s) {
   const float z = s * s;
   return s * fmaf(z, fmaf(z, fmaf(z, fmaf(z, p.cap_odd[4], p.cap_odd[3]), p.cap_odd[2]), p.cap_odd[1]), p.cap_odd[0]);
 }
+
+// Two FP32 values in one register pair, and the packed forms of the FMA pipe.
+SVL_DEV uint64_t two(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+SVL_DEV uint64_t two(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+SVL_DEV void apart(uint64_t v, uint32_t& lo, uint32_t& hi) { asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v)); }
+SVL_DEV uint64_t mul_two(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+SVL_DEV uint64_t add_two(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+SVL_DEV uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// capped_small over N values in place, eight at a time so that their chains
+// overlap.
+template <int N>
+SVL_DEV void capped_small(const AttnParams& p, uint32_t* w) {
+  uint64_t k[5];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) k[i] = two(p.cap_odd[i], p.cap_odd[i]);
+#pragma unroll
+  for (int c = 0; c < N; c += 8) {
+    uint64_t s[4], z[4], r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = two(w[c + 2 * i], w[c + 2 * i + 1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = mul_two(s[i], s[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = fma_two(z[i], k[4], k[3]);
+#pragma unroll
+    for (int j = 2; j >= 0; --j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = fma_two(z[i], r[i], k[j]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) apart(mul_two(s[i], r[i]), w[c + 2 * i], w[c + 2 * i + 1]);
+  }
+}
+
 // cap - 2 cap / (1 + e^2y); arg = 2 log2(e) scale / cap, cap2 = cap log2(e)
 SVL_DEV float capped_any(float s, float arg, float cap2) {
   return cap2 - __fdividef(2.0f * cap2, 1.0f + ex2_approx(s * arg));
@@ -37,15 +91,26 @@ SVL_DEV uint32_t pack2(__nv_bfloat16, float lo, float hi) {
   return r;
 }
 
+// Keeps the larger magnitudes of each half; NaN stays.
+SVL_DEV uint32_t max_abs(__half, uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("{\n.reg .b32 t;\nabs.f16x2 t, %2;\nmax.NaN.f16x2 %0, %1, t;\n}" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+SVL_DEV uint32_t max_abs(__nv_bfloat16, uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("{\n.reg .b32 t;\nabs.bf16x2 t, %2;\nmax.NaN.bf16x2 %0, %1, t;\n}" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // Per packed pair: the sign bit of each half whose exponent is all ones.
 SVL_DEV uint32_t non_finite(__half, uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
 SVL_DEV uint32_t non_finite(__nv_bfloat16, uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
 
 struct RingPos {
   uint32_t stage = 0, phase = 0;
-  template <int N>
-  SVL_DEV void next() {
-    if (++stage == N) {
+  SVL_DEV void next(uint32_t stages) {
+    if (++stage == stages) {
       stage = 0;
       phase ^= 1;
     }
@@ -53,11 +118,10 @@ struct RingPos {
 };
 
 // A position `slabs` further on (less than a turn).
-template <int N>
-SVL_DEV RingPos ahead(RingPos p, uint32_t slabs) {
+SVL_DEV RingPos ahead(RingPos p, uint32_t slabs, uint32_t stages) {
   p.stage += slabs;
-  if (p.stage >= N) {
-    p.stage -= N;
+  if (p.stage >= stages) {
+    p.stage -= stages;
     p.phase ^= 1;
   }
   return p;

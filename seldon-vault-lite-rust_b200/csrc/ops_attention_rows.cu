@@ -81,7 +81,7 @@ struct Feeder {
     tma_load_3d(ring + pos.stage * kSlabBytes, slab < slabs ? k : v, &full[pos.stage],
                 (int32_t)(slab < slabs ? slab : slab - slabs) * kSlabCols, kvh, row);
     ++issued;
-    pos.next<STAGES>();
+    pos.next(STAGES);
     if (++slab == 2 * slabs) {
       slab = 0;
       ++entry;
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto done = [&]() {
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.empty[pos.stage]);
-    pos.next<kStages>();
+    pos.next(kStages);
     ++at;
   };
 
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     RingPos back;
     for (uint32_t i = 0; i < feeder.issued; ++i) {
       if (i + kStages >= feeder.issued) mbar_wait(&sm.full[back.stage], back.phase, p.err);
-      back.next<kStages>();
+      back.next(kStages);
     }
   }
 }

@@ -59,6 +59,9 @@ static_assert(sizeof(Smem<64>) + 1024 <= kSmemLimit && sizeof(Smem<128>) + 1024 
                   sizeof(Smem<256>) + 1024 <= kSmemLimit,
               "shared memory");
 
+// The low `n` bits (none for n <= 0, all for n >= 32).
+SVL_DEV uint32_t bits_below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }
+
 // kind::f16 with A in tensor memory.
 SVL_DEV void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -77,14 +80,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                         const uint32_t tile_rows) {
   using Sh = Shape<HDP>;
-  constexpr int kTiles = Sh::kRowTiles, kStages = Sh::kStages, kAhead = Sh::kAhead;
+  constexpr int kTiles = Sh::kRowTiles, kAhead = Sh::kAhead;
   const int slabs = (p.head_dim + kSlabCols - 1) / kSlabCols;  // of a K or V tile
+  const uint32_t stages = Sh::kStages / slabs * slabs;          // whole tiles: theirs lie in one piece
   extern __shared__ uint8_t raw[];
   Smem<HDP>& sm = *(Smem<HDP>*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < (int)stages; ++i) {
       mbar_init(&sm.full[i], 1);
       mbar_init(&sm.empty[i], 1);
     }
@@ -131,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_expect_tx(&sm.full[pos.stage], kSlabBytes);
           tma_load_3d(sm.ring + pos.stage * kSlabBytes, map, &sm.full[pos.stage], s * kSlabCols, (int32_t)kvh, (int32_t)row);
           ++issued;
-          pos.next<kStages>();
+          pos.next(stages);
         }
       };
       for (uint32_t is = seg0; ok && is < seg1; ++is) {
@@ -161,8 +165,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // copies in flight land before the CTA leaves
         RingPos back;
         for (uint32_t i = 0; i < issued; ++i) {
-          if (i + kStages >= issued) mbar_wait(&sm.full[back.stage], back.phase, p.err);
-          back.next<kStages>();
+          if (i + stages >= issued) mbar_wait(&sm.full[back.stage], back.phase, p.err);
+          back.next(stages);
         }
         if (n_segs) mbar_wait(&sm.q_full, (n_segs - 1) & 1, p.err);
       }
@@ -176,50 +180,47 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t n_segs = 0, n_checks = 0;
       uint32_t taken[2] = {0, 0};  // p_ready phases
       bool ok = true;
-      auto steps = [&](int slab) { return min(4, max(0, (int)(hd + 15 - slab * kSlabCols) / 16)); };  // of 16 columns
+      const int k_steps = (hd + 15) / 16;
+      const uint32_t idesc_o = idesc_f16(128, k_steps * 16, 1) | kType;
+      // shared-memory descriptors at the first byte; addresses go in in 16s
+      const uint64_t q_desc = sdesc(q_smem, 16, 1024, kLayoutSW128), k_desc = sdesc(ring_smem, 16, 1024, kLayoutSW128);
+      // V, keys by columns: 64 columns a slab, 16 keys (2 KB) a step
+      const uint64_t v_desc = sdesc(ring_smem, kSlabBytes, 1024, kLayoutSW128);
       auto scores = [&](int t, int buf, RingPos at, bool release) {
-        for (int c = 0; ok && c < slabs; ++c) {
+        uint64_t a = q_desc + t * (Sh::kSlabs * kSlabBytes / 16), b = k_desc + at.stage * (kSlabBytes / 16);
+        for (int c = 0; c < slabs; ++c, a += kSlabBytes / 16, b += kSlabBytes / 16) {
           if (!mbar_wait(&sm.full[at.stage], at.phase, p.err)) {
             ok = false;
             return;
           }
           tc_fence_after();
-          const uint32_t a = q_smem + (t * Sh::kSlabs + c) * kSlabBytes, b = ring_smem + at.stage * kSlabBytes;
-          const int n = steps(c);
-          for (int k = 0; k < n; ++k)
-            mma_f16(tmem + buf * 128, sdesc(a + k * 32, 16, 1024, kLayoutSW128), sdesc(b + k * 32, 16, 1024, kLayoutSW128),
-                    idesc_s, (c | k) != 0);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (c * 4 + k < k_steps) mma_f16(tmem + buf * 128, a + k * 2, b + k * 2, idesc_s, (c | k) != 0);
           if (release) mma_commit(&sm.empty[at.stage]);
-          at.next<kStages>();
+          at.next(stages);
         }
         mma_commit(&sm.s_full[buf]);
       };
       auto outputs = [&](int t, int buf, RingPos at, bool accumulate, bool release) {
-        for (int c = 0; ok && c < slabs; ++c) {
-          if (!mbar_wait(&sm.full[at.stage], at.phase, p.err)) {
+        const uint64_t b = v_desc + at.stage * (kSlabBytes / 16);
+        for (int c = 0; c < slabs; ++c)
+          if (!mbar_wait(&sm.full[at.stage + c], at.phase, p.err)) {
             ok = false;
             return;
           }
-          tc_fence_after();
-          const uint32_t v = ring_smem + at.stage * kSlabBytes;
-          const uint32_t d = tmem + Sh::kOutTmem + t * HDP + c * kSlabCols;
-          const int n = steps(c);
-          if (n) {
-            const uint32_t idesc_o = idesc_f16(128, n * 16, 1) | kType;
+        tc_fence_after();
+        const uint32_t d = tmem + Sh::kOutTmem + t * HDP;
 #pragma unroll
-            for (int k = 0; k < 8; ++k)  // 16 keys each
-              mma_f16_ts(d, tmem + buf * 128 + k * 8, sdesc(v + k * 2048, kSlabBytes, 1024, kLayoutSW128), idesc_o,
-                         accumulate || k);
-          }
-          if (release) mma_commit(&sm.empty[at.stage]);
-          at.next<kStages>();
-        }
+        for (int k = 0; k < 8; ++k) mma_f16_ts(d, tmem + buf * 128 + k * 8, b + k * 128, idesc_o, accumulate || k);
+        if (release)
+          for (int c = 0; c < slabs; ++c) mma_commit(&sm.empty[at.stage + c]);
         mma_commit(&sm.pv_done[buf]);
       };
       // Asks the check warps for a V tile at `at`, once it is there.
       auto ask = [&](RingPos at) {
         for (int c = 0; ok && c < slabs; ++c) {
-          const RingPos slab = ahead<kStages>(at, c);
+          const RingPos slab = ahead(at, c, stages);
           if (!mbar_wait(&sm.full[slab.stage], slab.phase, p.err)) ok = false;
         }
         if (!ok) return;
@@ -251,10 +252,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int t = 0; t < 2; ++t)
             if (sees_any(e, t)) scores(t, t, pos, t == 1 || !sees_any(e, 1));
           if (n == 1) mma_commit(&sm.q_empty);
-          pos = ahead<kStages>(pos, slabs);
+          pos = ahead(pos, slabs, stages);
           for (uint32_t j = 0; ok && j < n; ++j) {
             const uint32_t e2 = j + 2 < n ? list[j + 2] : 0;  // in flight under this tile's waits
-            const RingPos v = pos, k = ahead<kStages>(pos, slabs);
+            const RingPos v = pos, k = ahead(pos, slabs, stages);
             const bool more = j + 1 < n;
             if (some(e)) {
               ask(v);
@@ -272,16 +273,16 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (more && sees_any(e1, t)) scores(t, t, k, t == 1 || !sees_any(e1, 1));
             }
             if (j + 2 == n) mma_commit(&sm.q_empty);
-            pos = ahead<kStages>(pos, more ? 2 * slabs : slabs);
+            pos = ahead(pos, more ? 2 * slabs : slabs, stages);
             e = e1;
             e1 = e2;
           }
         } else {
           scores(0, g & 1, pos, true);
-          pos = ahead<kStages>(pos, slabs);
+          pos = ahead(pos, slabs, stages);
           if (n > 1) {
             scores(0, (g + 1) & 1, pos, true);
-            pos = ahead<kStages>(pos, slabs);
+            pos = ahead(pos, slabs, stages);
           }
           if (n <= 2) mma_commit(&sm.q_empty);
           for (uint32_t j = 0; ok && j < n; ++j, ++g) {
@@ -296,10 +297,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             tc_fence_after();
             outputs(0, buf, pos, j > 0, true);
-            pos = ahead<kStages>(pos, slabs);
+            pos = ahead(pos, slabs, stages);
             if (j + 2 < n) {
               scores(0, buf, pos, true);
-              pos = ahead<kStages>(pos, slabs);
+              pos = ahead(pos, slabs, stages);
               if (j + 3 == n) mma_commit(&sm.q_empty);
             }
             e = e1;
@@ -333,17 +334,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < slabs; ++c) {
           mbar_wait(&sm.full[at.stage], at.phase, p.err);  // passed already: orders this thread's reads
           uint4* slab = (uint4*)(sm.ring + at.stage * kSlabBytes);
-#pragma unroll 4
-          for (int i = tid; i < kSlabBytes / 16; i += 64) {
-            const uint4 w = slab[i];
-            const uint32_t b[4] = {non_finite(T(), w.x), non_finite(T(), w.y), non_finite(T(), w.z), non_finite(T(), w.w)};
-            if (b[0] | b[1] | b[2] | b[3]) {
-              found = true;
-              auto zero = [](uint32_t x, uint32_t bad) { return x & ~((bad >> 15) * 0xffffu); };
-              slab[i] = make_uint4(zero(w.x, b[0]), zero(w.y, b[1]), zero(w.z, b[2]), zero(w.w, b[3]));
+          uint32_t most[4] = {};
+#pragma unroll 8
+          for (int i = 0; i < kSlabBytes / 16 / 64; ++i) {
+            const uint4 w = slab[i * 64 + tid];
+            most[0] = max_abs(T(), most[0], w.x);
+            most[1] = max_abs(T(), most[1], w.y);
+            most[2] = max_abs(T(), most[2], w.z);
+            most[3] = max_abs(T(), most[3], w.w);
+          }
+          if (non_finite(T(), most[0]) | non_finite(T(), most[1]) | non_finite(T(), most[2]) | non_finite(T(), most[3])) {
+            found = true;
+#pragma unroll 1
+            for (int i = 0; i < kSlabBytes / 16 / 64; ++i) {
+              const uint4 w = slab[i * 64 + tid];
+              auto zero = [](uint32_t x) { return x & ~((non_finite(T(), x) >> 15) * 0xffffu); };
+              slab[i * 64 + tid] = make_uint4(zero(w.x), zero(w.y), zero(w.z), zero(w.w));
             }
           }
-          at.next<kStages>();
+          at.next(stages);
         }
         if (found) sm.spoiled[mail.segment & 1] = mail.segment;
         fence_async_smem();
@@ -424,34 +433,58 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int c = 0; c < kCols; ++c) w[c] = __float_as_uint(capped_any(x(c), cap_arg, cap2));
           } else {
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) w[c] = __float_as_uint(capped_small(p, x(c)));
+            capped_small<kCols>(p, w);
           }
-        } else if (biased) {
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) w[c] = __float_as_uint(x(c) * scale2);
         }
         if (biased) {
-          const float gap = (float)(mask.place - j0);
+          const float gap = (float)(mask.place - j0), by = capped ? 1.0f : scale2;
+          // the distance |gap - c| is linear in c unless the row's own place lies inside the tile
+          if (__all_sync(0xffffffffu, gap >= (float)(kCols - 1) || gap <= 0.0f)) {
+            const float rise = gap > 0.0f ? slope2 : -slope2;
+            const uint64_t by2 = two(by, by), rise2 = two(rise, rise), start2 = two(-rise * gap, -rise * gap);
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) w[c] = __float_as_uint(fmaf(-slope2, fabsf(gap - (float)c), x(c)));
+            for (int c = 0; c < kCols; c += 8) {
+              uint64_t t2[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) t2[i] = fma_two(rise2, two((float)(c + 2 * i), (float)(c + 2 * i + 1)), start2);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                apart(fma_two(two(w[c + 2 * i], w[c + 2 * i + 1]), by2, t2[i]), w[c + 2 * i], w[c + 2 * i + 1]);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) w[c] = __float_as_uint(fmaf(x(c), by, -slope2 * fabsf(gap - (float)c)));
+          }
         }
         if (see == kSeesSome) {
           const int lo = (int)max((int64_t)0, min(first - j0, (int64_t)kCols));
           const int hi = (int)max((int64_t)-1, min(last - j0, (int64_t)kCols - 1));
           const int pre = (int)max((int64_t)0, min((int64_t)prefix - j0, (int64_t)kCols));
-          if (p.doc_k) {
-            const int n = (int)max((int64_t)0, min((int64_t)s.n_k - j0, (int64_t)kCols));
-            const int32_t* docs = p.doc_k + s.k0 + j0;
+          const int n = (int)max((int64_t)0, min((int64_t)s.n_k - j0, (int64_t)kCols));
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-              const int32_t d = c < n ? __ldg(docs + c) : -1;
-              if (!(d >= 0 && (c < pre || (c >= lo && c <= hi && d == mask.doc)))) w[c] = __float_as_uint(-INFINITY);
+          for (int c = 0; c < kCols; c += 32) {
+            // one bit a key
+            uint32_t bits = bits_below(hi + 1 - c) & ~bits_below(lo - c);
+            const uint32_t ahead = bits_below(pre - c);
+            if (p.doc_k) {
+              // a lane loads a key's document; each document of the 32 in turn gives its keys to its rows
+              const int32_t d = c + lane < n ? __ldg(p.doc_k + s.k0 + j0 + c + lane) : -1;
+              const uint32_t member = __ballot_sync(0xffffffffu, d >= 0);
+              uint32_t own = 0;
+              for (uint32_t left = member; left;) {
+                const int32_t one = __shfl_sync(0xffffffffu, d, __ffs(left) - 1);
+                const uint32_t its = __ballot_sync(0xffffffffu, d == one);
+                if (one == mask.doc) own = its;
+                left &= ~its;
+              }
+              bits = (ahead | (bits & own)) & member;
+            } else {
+              bits |= ahead;
             }
-          } else {
+            if (__all_sync(0xffffffffu, bits == 0xffffffffu)) continue;
 #pragma unroll
-            for (int c = 0; c < kCols; ++c)
-              if (!(c < pre || (c >= lo && c <= hi))) w[c] = __float_as_uint(-INFINITY);
+            for (int i = 0; i < 32; ++i)
+              if (!(bits >> i & 1)) w[c + i] = __float_as_uint(-INFINITY);
           }
         }
         float mx[4];
@@ -492,19 +525,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         started = true;
         __syncwarp();
         const float base = m == -INFINITY ? 0.0f : m * unit;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint64_t unit2 = two(unit, unit), base2 = two(-base, -base);
+        uint64_t sum[4] = {0, 0, 0, 0};  // pairs of 0.0f
 #pragma unroll
         for (int c = 0; c < kCols; c += 32) {
           uint32_t pk[16];
 #pragma unroll
-          for (int u = 0; u < 16; ++u) {
-            const float a = ex2_approx(fmaf(x(c + 2 * u), unit, -base)), b = ex2_approx(fmaf(x(c + 2 * u + 1), unit, -base));
-            sum[u & 3] += a + b;
-            pk[u] = pack2(T(), a, b);
+          for (int u = 0; u < 16; u += 4) {
+            uint64_t y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = fma_two(two(w[c + 2 * (u + i)], w[c + 2 * (u + i) + 1]), unit2, base2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t a, b;
+              apart(y[i], a, b);
+              const float ea = ex2_approx(__uint_as_float(a)), eb = ex2_approx(__uint_as_float(b));
+              sum[i] = add_two(sum[i], two(ea, eb));
+              pk[u + i] = pack2(T(), ea, eb);
+            }
           }
           tmem_st16(s_addr + (half * kCols + c) / 2, pk);
         }
-        l = l * factor + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        uint32_t part[2];
+        apart(add_two(add_two(sum[0], sum[1]), add_two(sum[2], sum[3])), part[0], part[1]);
+        l = l * factor + (__uint_as_float(part[0]) + __uint_as_float(part[1]));
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
