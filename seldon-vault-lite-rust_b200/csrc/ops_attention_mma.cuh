@@ -15,10 +15,10 @@ constexpr float kBehind = 8.0f;  // a maximum follows once it is 2^8 behind (log
 
 // cap tanh(scale s / cap) of a raw score s in log2 units.  tanh y = y P(y^2) with
 // P of degree 4 fitted to tanh(y) / y for |y| <= 1/2 (relative error 1.3e-8, below
-// FP32's half step): five multiply-adds on the FMA pipe, with the cap and scale
-// in the coefficients.  The general form costs two of the 16 special functions a
-// cycle that the softmax itself needs; a warp takes it when a score of its tile
-// lies behind cap_limit = cap / (2 scale).
+// FP32's half step): multiply-adds on the FMA pipe, with the cap and scale in the
+// coefficients.  The general form costs two of the 16 special functions a cycle
+// that the softmax itself needs; a warp takes it when a score of its tile lies
+// behind cap_limit = cap / (2 scale).
 constexpr double kTanhOdd[5] = {0.9999999873738349, -0.33333075792040845, 0.133249069544671, -0.052994230404600086,
                                 0.017151297500408665};
 SVL_DEV float capped_small(const AttnParams& p, float s) {
@@ -54,18 +54,15 @@ SVL_DEV uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// capped_small over N values in place, eight at a time so that their chains
-// overlap.
-template <int N>
-SVL_DEV void capped_small(const AttnParams& p, uint32_t* w) {
+// P of four pairs.
+struct CapOdd {
   uint64_t k[5];
+  SVL_DEV CapOdd(const AttnParams& p) {
 #pragma unroll
-  for (int i = 0; i < 5; ++i) k[i] = two(p.cap_odd[i], p.cap_odd[i]);
-#pragma unroll
-  for (int c = 0; c < N; c += 8) {
-    uint64_t s[4], z[4], r[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = two(w[c + 2 * i], w[c + 2 * i + 1]);
+    for (int i = 0; i < 5; ++i) k[i] = two(p.cap_odd[i], p.cap_odd[i]);
+  }
+  SVL_DEV void over(const uint64_t* s, uint64_t* r) const {
+    uint64_t z[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) z[i] = mul_two(s[i], s[i]);
 #pragma unroll
@@ -74,6 +71,20 @@ SVL_DEV void capped_small(const AttnParams& p, uint32_t* w) {
     for (int j = 2; j >= 0; --j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) r[i] = fma_two(z[i], r[i], k[j]);
+  }
+};
+
+// capped_small over N values in place, eight at a time so that their chains
+// overlap.
+template <int N>
+SVL_DEV void capped_small(const AttnParams& p, uint32_t* w) {
+  const CapOdd odd(p);
+#pragma unroll
+  for (int c = 0; c < N; c += 8) {
+    uint64_t s[4], r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = two(w[c + 2 * i], w[c + 2 * i + 1]);
+    odd.over(s, r);
 #pragma unroll
     for (int i = 0; i < 4; ++i) apart(mul_two(s[i], r[i]), w[c + 2 * i], w[c + 2 * i + 1]);
   }

@@ -2,15 +2,17 @@
 // on the 5th-generation tensor cores.
 //
 // One persistent CTA per SM walks its segments (rows of one key-value head
-// against a list of 128-key tiles).  A row tile is up to 128 (query, head of
-// the group) rows, so every head of a group reads a key tile once.  Head
-// sizes up to 128: two row tiles share each key tile, one softmax warpgroup
-// each, so that one tile's products run under the other's softmax.  Head sizes
-// up to 256: one row tile with two score buffers, its 128 columns split between
-// the two warpgroups.
+// against a list of 128-key tiles).  A row tile is up to 128 (query, head of the
+// group) rows, so every head of a group reads a key tile once.  Head sizes up to
+// 128: two row tiles share each key tile, so that one tile's products run under
+// the other's softmax.  Head sizes up to 256: one row tile with two score
+// buffers.  Two softmax warpgroups share a row tile, 64 of a key tile's columns
+// each: with one of them a scheduler has a single softmax warp for each row tile,
+// whose chains of dependent instructions it cannot fill (622 against UNMEASURED us for
+// the 8192-token prefix case).
 //
 //   S = Q K^T  128 x 128 into TMEM (kind::f16, FP32 accumulators)
-//   softmax    one row per thread: running maximum m and sum l; weights
+//   softmax    half a row per thread: running maximum m and sum l; weights
 //              P = 2^(t - m) rounded to the type over S's own columns.  m
 //              follows the row's maximum only once it is more than 2^8 behind,
 //              so O is rarely rescaled; the weights stay below 2^8.
@@ -26,18 +28,22 @@
 namespace svl {
 namespace {
 
-constexpr int kThreads = 384;  // warpgroup 0: loads, MMAs, checks; 1 and 2: softmax
-constexpr int kRegsControl = 72, kRegsSoftmax = 216;  // 72 + 2 * 216 = 3 * 168
+constexpr int kCols = 64;  // score columns of a softmax thread
 
 template <int HDP>
 struct Shape {
   static constexpr int kRowTiles = HDP <= 128 ? 2 : 1;
   static constexpr int kAhead = HDP <= 128 ? 1 : 2;       // score tiles of a row tile in flight
   static constexpr int kSlabs = HDP / kSlabCols;          // of a K or V tile
-  static constexpr int kStages = HDP == 64 ? 12 : HDP == 128 ? 10 : 9;
-  static constexpr int kCols = 128 / (3 - kRowTiles);     // score columns of a softmax thread
-  static constexpr int kOutCols = kRowTiles == 2 ? HDP : HDP / 2;  // output columns of a softmax thread
+  static constexpr int kStages = HDP == 64 ? 11 : 9;
+  static constexpr int kOutCols = HDP / 2;                // output columns of a softmax thread
   static constexpr uint32_t kOutTmem = 256;
+  // warpgroup 0: loads, MMAs, checks; the others: softmax
+  static constexpr int kSoftmax = 2 * kRowTiles, kThreads = 128 * (1 + kSoftmax);
+  static constexpr int kRegs = kRowTiles == 2 ? 96 : 168;  // of a thread at launch: 65536 / kThreads, in eights
+  static constexpr int kRegsControl = kRowTiles == 2 ? 64 : 72;
+  static constexpr int kRegsSoftmax = kRowTiles == 2 ? 104 : 216;
+  static_assert(kRegsControl + kSoftmax * kRegsSoftmax == (1 + kSoftmax) * kRegs, "registers move inside the launch's own");
 };
 
 struct Mailbox {
@@ -53,11 +59,35 @@ struct Smem {
   uint32_t tmem;
   Mailbox mail;
   uint32_t spoiled[2];  // 1 + the CTA's last segment of that parity with non-finite values
-  float row_max[HDP > 128 ? 2 : 1][2][HDP > 128 ? 128 : 1];
+  float shared_row[2][Shape<HDP>::kRowTiles][2][128];  // [parity][row tile][half]: maxima, sums
 };
 static_assert(sizeof(Smem<64>) + 1024 <= kSmemLimit && sizeof(Smem<128>) + 1024 <= kSmemLimit &&
                   sizeof(Smem<256>) + 1024 <= kSmemLimit,
               "shared memory");
+
+// A step of the transposition of four lanes' four units: lanes l and l ^ D swap
+// the off-diagonal blocks of theirs.
+template <int D>
+SVL_DEV void exchange(uint4* v, int lane) {
+  const bool upper = lane & D;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    if (u & D) continue;
+    uint4 give = upper ? v[u] : v[u | D];
+    give.x = __shfl_xor_sync(0xffffffffu, give.x, D);
+    give.y = __shfl_xor_sync(0xffffffffu, give.y, D);
+    give.z = __shfl_xor_sync(0xffffffffu, give.z, D);
+    give.w = __shfl_xor_sync(0xffffffffu, give.w, D);
+    if (upper) v[u] = give;
+    else v[u | D] = give;
+  }
+}
+
+SVL_DEV float fmin3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // The low `n` bits (none for n <= 0, all for n >= 32).
 SVL_DEV uint32_t bits_below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }
@@ -75,7 +105,7 @@ SVL_DEV void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32
 SVL_DEV void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 template <typename T, int HDP>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
     attention_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap map_q,
                         const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                         const uint32_t tile_rows) {
@@ -97,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&sm.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_ready[i], kTiles == 2 ? 4 : 8);
+      mbar_init(&sm.p_ready[i], 8);
       mbar_init(&sm.pv_done[i], 1);
     }
     mbar_init(&sm.check_req, 1);
@@ -119,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t seg0 = p.block_segments[blockIdx.x], seg1 = p.block_segments[blockIdx.x + 1];
 
   if (warp < 4) {
-    setmaxnreg_dec<kRegsControl>();
+    setmaxnreg_dec<Sh::kRegsControl>();
     if (warp == 0 && lane == 0) {
       // ------------------------------------------------------------- loads --
       const uint32_t q_bytes = tile_rows * 128;  // of one slab
@@ -212,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t d = tmem + Sh::kOutTmem + t * HDP;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) mma_f16_ts(d, tmem + buf * 128 + k * 8, b + k * 128, idesc_o, accumulate || k);
+        for (int k = 0; k < 8; ++k) mma_f16_ts(d, tmem + buf * 128 + k / 4 * kCols + k % 4 * 8, b + k * 128, idesc_o, accumulate || k);
         if (release)
           for (int c = 0; c < slabs; ++c) mma_commit(&sm.empty[at.stage + c]);
         mma_commit(&sm.pv_done[buf]);
@@ -361,19 +391,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // -------------------------------------------------------------- softmax --
-    setmaxnreg_inc<kRegsSoftmax>();
+    setmaxnreg_inc<Sh::kRegsSoftmax>();
     const int wg = (warp - 4) >> 2, lg = warp & 3;
-    const int t = kTiles == 2 ? wg : 0;        // row tile
-    const int half = kTiles == 2 ? 0 : wg;     // column half
+    const int t = wg >> 1, half = wg & 1;  // row tile, columns
     const int r = lg * 32 + lane;
+    const int pair = 1 + t * 4 + lg;       // the barrier of the two warps of these rows
     const uint32_t lane_addr = tmem + ((uint32_t)(lg * 32) << 16);
-    const uint32_t out_addr = lane_addr + Sh::kOutTmem + (kTiles == 2 ? t * HDP : half * Sh::kOutCols);
-    constexpr int kCols = Sh::kCols;
+    const uint32_t out_addr = lane_addr + Sh::kOutTmem + t * HDP + half * Sh::kOutCols;
     const bool capped = p.cap > 0.0f, biased = p.slopes != nullptr, plain = !capped && !biased;
     const float scale2 = p.scale * kLog2e;
-    const float unit = plain ? scale2 : 1.0f;  // log2 units of a score as it is kept
     const float cap2 = p.cap * kLog2e, cap_arg = capped ? 2.0f * scale2 / p.cap : 0.0f;
-    const float behind = kBehind / unit;
     uint32_t g = 0;       // tiles of this warpgroup
     uint32_t n_segs = 0;
     bool dead = false;    // a wait ran out: no more waits, but every step is taken
@@ -414,61 +441,104 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t see = entry_sees(e, t);
         if (see == kSeesNone) continue;
         const int buf = kTiles == 2 ? t : (int)(g & 1);
+        const int64_t j0 = (int64_t)entry_tile(e) * kKeyTile + half * kCols;
+        // a lane loads two keys' documents, under the wait for the scores
+        int32_t docs[2] = {-1, -1};
+        if (p.doc_k && see == kSeesSome) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (j0 + 32 * h + lane < (int64_t)s.n_k) docs[h] = __ldg(p.doc_k + s.k0 + j0 + 32 * h + lane);
+        }
         wait(&sm.s_full[buf], (kTiles == 2 ? g : g >> 1) & 1);
         tc_fence_after();
-        const uint32_t s_addr = lane_addr + buf * 128;
-        uint32_t w[kCols];
+        const uint32_t s_addr = lane_addr + buf * 128 + half * kCols;
+        // Tiles that a row sees whole need nothing but the maximum (and, for the
+        // cap, the minimum) here, and their scores are transformed where they are
+        // exponentiated.  The distance is linear over columns that the row's own
+        // place does not lie among.  In all other cases the transformed scores go
+        // back to TMEM.
+        const float gap = (float)(mask.place - j0);
+        const bool apart_from = gap >= (float)(kCols - 1) || gap <= 0.0f;
+        const bool direct = see == kSeesAll && (plain || (capped != biased && (capped || __all_sync(0xffffffffu, apart_from))));
+        const float rise = gap > 0.0f ? slope2 : -slope2;  // direct bias: -slope |gap - c| = rise (c - gap)
+        float top = -INFINITY;
+        bool small = true;  // every score within the cap's polynomial
+        if (direct) {
+          float low = INFINITY;
+#pragma unroll 1
+          for (int c0 = 0; c0 < kCols; c0 += 32) {
+            uint32_t w[32];
+            tmem_ld32_nowait(s_addr + c0, w);
+            tmem_ld_wait();
+            tmem_regs_after_wait(w);
+            auto x = [&](int c) { return __uint_as_float(w[c]); };
+            if (biased) {
+              const uint64_t by2 = two(scale2, scale2), rise2 = two(2.0f * rise, 2.0f * rise);
+              uint64_t t2 = two(rise * ((float)c0 - gap), rise * ((float)c0 - gap) + rise);
 #pragma unroll
-        for (int c = 0; c < kCols / 32; ++c) tmem_ld32_nowait(s_addr + half * kCols + c * 32, w + c * 32);
-        tmem_ld_wait();
-#pragma unroll
-        for (int c = 0; c < kCols / 32; ++c) tmem_regs_after_wait(w + c * 32);
-        auto x = [&](int c) { return __uint_as_float(w[c]); };
-        const int64_t j0 = (int64_t)entry_tile(e) * kKeyTile + half * kCols;
-        if (capped) {
-          float most = 0.0f;
-#pragma unroll
-          for (int c = 0; c < kCols; c += 2) most = fmax3(most, fabsf(x(c)), fabsf(x(c + 1)));
-          if (__any_sync(0xffffffffu, most > p.cap_limit)) {
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) w[c] = __float_as_uint(capped_any(x(c), cap_arg, cap2));
-          } else {
-            capped_small<kCols>(p, w);
-          }
-        }
-        if (biased) {
-          const float gap = (float)(mask.place - j0), by = capped ? 1.0f : scale2;
-          // the distance |gap - c| is linear in c unless the row's own place lies inside the tile
-          if (__all_sync(0xffffffffu, gap >= (float)(kCols - 1) || gap <= 0.0f)) {
-            const float rise = gap > 0.0f ? slope2 : -slope2;
-            const uint64_t by2 = two(by, by), rise2 = two(rise, rise), start2 = two(-rise * gap, -rise * gap);
-#pragma unroll
-            for (int c = 0; c < kCols; c += 8) {
-              uint64_t t2[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) t2[i] = fma_two(rise2, two((float)(c + 2 * i), (float)(c + 2 * i + 1)), start2);
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                apart(fma_two(two(w[c + 2 * i], w[c + 2 * i + 1]), by2, t2[i]), w[c + 2 * i], w[c + 2 * i + 1]);
+              for (int c = 0; c < 32; c += 2) {
+                apart(fma_two(two(w[c], w[c + 1]), by2, t2), w[c], w[c + 1]);
+                t2 = add_two(t2, rise2);
+              }
             }
-          } else {
+            float mx[2] = {x(0), x(1)};
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) w[c] = __float_as_uint(fmaf(x(c), by, -slope2 * fabsf(gap - (float)c)));
+            for (int c = 2; c < 32; c += 4) {
+              mx[0] = fmax3(mx[0], x(c), x(c + 1));
+              if (c + 2 < 32) mx[1] = fmax3(mx[1], x(c + 2), x(c + 3));
+            }
+            top = fmax3(top, mx[0], mx[1]);
+            if (capped) {
+              float mn[2] = {x(0), x(1)};
+#pragma unroll
+              for (int c = 2; c < 32; c += 4) {
+                mn[0] = fmin3(mn[0], x(c), x(c + 1));
+                if (c + 2 < 32) mn[1] = fmin3(mn[1], x(c + 2), x(c + 3));
+              }
+              low = fmin3(low, mn[0], mn[1]);
+            }
           }
-        }
-        if (see == kSeesSome) {
-          const int lo = (int)max((int64_t)0, min(first - j0, (int64_t)kCols));
-          const int hi = (int)max((int64_t)-1, min(last - j0, (int64_t)kCols - 1));
-          const int pre = (int)max((int64_t)0, min((int64_t)prefix - j0, (int64_t)kCols));
-          const int n = (int)max((int64_t)0, min((int64_t)s.n_k - j0, (int64_t)kCols));
+          if (plain) top *= scale2;
+          if (capped) {
+            small = !__any_sync(0xffffffffu, fmaxf(top, -low) > p.cap_limit);
+            top = top == -INFINITY ? top : capped_any(top, cap_arg, cap2);  // the cap keeps the order
+          }
+        } else
+#pragma unroll 1
+        for (int c0 = 0; c0 < kCols; c0 += 32) {
+          uint32_t w[32];
+          tmem_ld32_nowait(s_addr + c0, w);
+          tmem_ld_wait();
+          tmem_regs_after_wait(w);
+          auto x = [&](int c) { return __uint_as_float(w[c]); };
+          if (capped) {
+            float most = 0.0f;
 #pragma unroll
-          for (int c = 0; c < kCols; c += 32) {
+            for (int c = 0; c < 32; c += 2) most = fmax3(most, fabsf(x(c)), fabsf(x(c + 1)));
+            if (__any_sync(0xffffffffu, most > p.cap_limit)) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c) w[c] = __float_as_uint(capped_any(x(c), cap_arg, cap2));
+            } else {
+              capped_small<32>(p, w);
+            }
+          }
+          if (biased) {
+            const float from = gap - (float)c0, by = capped ? 1.0f : scale2;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) w[c] = __float_as_uint(fmaf(x(c), by, -slope2 * fabsf(from - (float)c)));
+          } else if (!capped) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) w[c] = __float_as_uint(x(c) * scale2);
+          }
+          if (see == kSeesSome) {
+            const int64_t j = j0 + c0;
             // one bit a key
-            uint32_t bits = bits_below(hi + 1 - c) & ~bits_below(lo - c);
-            const uint32_t ahead = bits_below(pre - c);
+            uint32_t bits = bits_below((int)max((int64_t)0, min(last + 1 - j, (int64_t)32))) &
+                            ~bits_below((int)max((int64_t)0, min(first - j, (int64_t)32)));
+            const uint32_t ahead = bits_below((int)max((int64_t)0, min((int64_t)prefix - j, (int64_t)32)));
             if (p.doc_k) {
-              // a lane loads a key's document; each document of the 32 in turn gives its keys to its rows
-              const int32_t d = c + lane < n ? __ldg(p.doc_k + s.k0 + j0 + c + lane) : -1;
+              // each document of the 32 in turn gives its keys to its rows
+              const int32_t d = c0 ? docs[1] : docs[0];
               const uint32_t member = __ballot_sync(0xffffffffu, d >= 0);
               uint32_t own = 0;
               for (uint32_t left = member; left;) {
@@ -481,33 +551,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
               bits |= ahead;
             }
-            if (__all_sync(0xffffffffu, bits == 0xffffffffu)) continue;
+            if (!__all_sync(0xffffffffu, bits == 0xffffffffu)) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(bits >> i & 1)) w[c + i] = __float_as_uint(-INFINITY);
+              for (int i = 0; i < 32; ++i)
+                if (!(bits >> i & 1)) w[i] = __float_as_uint(-INFINITY);
+            }
           }
-        }
-        float mx[4];
+          float mx[2] = {x(0), x(1)};
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          constexpr int kPart = kCols / 4;
-          mx[u] = x(u * kPart);
-#pragma unroll
-          for (int c = 1; c + 1 < kPart; c += 2) mx[u] = fmax3(mx[u], x(u * kPart + c), x(u * kPart + c + 1));
-          mx[u] = fmaxf(mx[u], x(u * kPart + kPart - 1));
+          for (int c = 2; c < 32; c += 4) {
+            mx[0] = fmax3(mx[0], x(c), x(c + 1));
+            if (c + 2 < 32) mx[1] = fmax3(mx[1], x(c + 2), x(c + 3));
+          }
+          top = fmax3(top, mx[0], mx[1]);
+          __syncwarp();
+          tmem_st32(s_addr + c0, w);
+          tmem_st_wait();
         }
-        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        if constexpr (kTiles == 1) {
-          // both halves of a row follow one maximum
-          sm.row_max[g & 1][half][r] = top;
-          tc_fence_before();  // both halves are read before either is written over
-          pair_sync(1 + lg);
-          tc_fence_after();
-          top = fmaxf(top, sm.row_max[g & 1][half ^ 1][r]);
-        }
+        // both halves of a row follow one maximum
+        sm.shared_row[g & 1][t][half][r] = top;
+        pair_sync(pair);
+        top = fmaxf(top, sm.shared_row[g & 1][t][half ^ 1][r]);
         float factor = 1.0f;
-        if (top > m + behind || (m == -INFINITY && top > -INFINITY)) {
-          factor = m == -INFINITY ? 0.0f : ex2_approx((m - top) * unit);
+        if (top > m + kBehind || (m == -INFINITY && top > -INFINITY)) {
+          factor = m == -INFINITY ? 0.0f : ex2_approx(m - top);
           m = top;
         }
         if (started && __any_sync(0xffffffffu, factor != 1.0f)) {
@@ -524,30 +591,79 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         started = true;
         __syncwarp();
-        const float base = m == -INFINITY ? 0.0f : m * unit;
-        const uint64_t unit2 = two(unit, unit), base2 = two(-base, -base);
-        uint64_t sum[4] = {0, 0, 0, 0};  // pairs of 0.0f
+        const float base = m == -INFINITY ? 0.0f : m;
+        uint64_t sum[2] = {0, 0};  // pairs of 0.0f
+        // 2^(t - m) of 32 columns; `exponents` makes four pairs of t - m from four of scores
+        auto weights = [&](auto&& exponents) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < kCols; c0 += 32) {
+            uint32_t w[32], pk[16];
+            tmem_ld32_nowait(s_addr + c0, w);
+            tmem_ld_wait();
+            tmem_regs_after_wait(w);
 #pragma unroll
-        for (int c = 0; c < kCols; c += 32) {
-          uint32_t pk[16];
+            for (int u = 0; u < 16; u += 4) {
+              uint64_t y[4];
 #pragma unroll
-          for (int u = 0; u < 16; u += 4) {
-            uint64_t y[4];
+              for (int i = 0; i < 4; ++i) y[i] = two(w[2 * (u + i)], w[2 * (u + i) + 1]);
+              exponents(y, c0 + 2 * u);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = fma_two(two(w[c + 2 * (u + i)], w[c + 2 * (u + i) + 1]), unit2, base2);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t a, b;
-              apart(y[i], a, b);
-              const float ea = ex2_approx(__uint_as_float(a)), eb = ex2_approx(__uint_as_float(b));
-              sum[i] = add_two(sum[i], two(ea, eb));
-              pk[u + i] = pack2(T(), ea, eb);
+              for (int i = 0; i < 4; ++i) {
+                uint32_t a, b;
+                apart(y[i], a, b);
+                const float ea = ex2_approx(__uint_as_float(a)), eb = ex2_approx(__uint_as_float(b));
+                sum[i & 1] = add_two(sum[i & 1], two(ea, eb));
+                pk[u + i] = pack2(T(), ea, eb);
+              }
             }
+            tmem_st16(s_addr + c0 / 2, pk);  // over what this warp has read of these columns
           }
-          tmem_st16(s_addr + (half * kCols + c) / 2, pk);
+        };
+        const uint64_t base2 = two(-base, -base);
+        if (!direct) {
+          weights([&](uint64_t* y, int) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = add_two(y[i], base2);
+          });
+        } else if (capped) {
+          if (small) {
+            const CapOdd odd(p);
+            weights([&](uint64_t* y, int) {
+              uint64_t r[4];
+              odd.over(y, r);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) y[i] = fma_two(y[i], r[i], base2);
+            });
+          } else {
+            weights([&](uint64_t* y, int) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint32_t a, b;
+                apart(y[i], a, b);
+                y[i] = two(capped_any(__uint_as_float(a), cap_arg, cap2) - base, capped_any(__uint_as_float(b), cap_arg, cap2) - base);
+              }
+            });
+          }
+        } else {
+          // biased: rise (c - gap); plain: no rise
+          const float up = biased ? rise : 0.0f, start = biased ? -rise * gap - base : -base;
+          const uint64_t by2 = two(scale2, scale2), up2 = two(2.0f * up, 2.0f * up);
+          weights([&](uint64_t* y, int c) {
+            if (biased) {
+              uint64_t t2 = two(fmaf(up, (float)c, start), fmaf(up, (float)(c + 1), start));
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                y[i] = fma_two(y[i], by2, t2);
+                t2 = add_two(t2, up2);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) y[i] = fma_two(y[i], by2, base2);
+            }
+          });
         }
         uint32_t part[2];
-        apart(add_two(add_two(sum[0], sum[1]), add_two(sum[2], sum[3])), part[0], part[1]);
+        apart(add_two(sum[0], sum[1]), part[0], part[1]);
         l = l * factor + (__uint_as_float(part[0]) + __uint_as_float(part[1]));
         tmem_st_wait();
         tc_fence_before();
@@ -556,28 +672,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++g;
       }
       // ------------------------------------------------------------ epilogue --
-      if constexpr (kTiles == 1) {
-        const int at = g & 1;  // the next tile writes the other parity's slot first
-        sm.row_max[at][half][r] = l;
-        pair_sync(1 + lg);
-        l += sm.row_max[at][half ^ 1][r];
-        pair_sync(1 + lg);
+      {
+        const int at = g & 1;  // not the last tile's slot, and the next tile writes this one after the barrier
+        sm.shared_row[at][t][half][r] = l;
+        pair_sync(pair);
+        l += sm.shared_row[at][t][half ^ 1][r];
+        pair_sync(pair);
       }
       if (started) product_done();
       tc_fence_after();
       const bool spoiled = started && sm.spoiled[n_segs & 1] == n_segs;
       const bool empty = !started || (m == -INFINITY && l == 0.0f);
       const float inv = empty ? 0.0f : 1.0f / l;
-      const float lse = empty ? -INFINITY : kLn2 * ((m == -INFINITY ? 0.0f : m * unit) + log2f(l));
+      const float lse = empty ? -INFINITY : kLn2 * ((m == -INFINITY ? 0.0f : m) + log2f(l));
       const uint64_t token = s.q0 + query;
       const uint64_t part = (uint64_t)(seg.slot < 0 ? 0 : seg.slot) * p.slot_rows + in_seg;
+      const uint64_t row_at = live ? token * p.ld_out + (uint64_t)head * p.head_dim : ~0ull;
       if (live && half == 0) {
         if (seg.slot >= 0) p.part_lse[part] = lse;
         else if (p.lse) p.lse[token * p.q_heads + head] = lse;
       }
 #pragma unroll 1
       for (int c = 0; c < Sh::kOutCols; c += 32) {
-        const uint32_t col0 = (kTiles == 1 ? half * Sh::kOutCols : 0) + c;
+        const uint32_t col0 = half * Sh::kOutCols + c;
         if (col0 >= p.head_dim) break;
         float o[32];
         if (started) {
@@ -598,13 +715,23 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int u = 0; u < 32; u += 4)
             if (col0 + u < p.head_dim) *(float4*)(dst + u) = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
-        } else if (live) {
-          T* dst = (T*)p.out + token * p.ld_out + (uint64_t)head * p.head_dim + col0;
+        }
+        if (seg.slot < 0) {
+          // Four lanes exchange their rows' 16-byte units, so that they write 64
+          // contiguous bytes of one row after another.
+          uint4 v[4];
 #pragma unroll
-          for (int u = 0; u < 32; u += 8)
-            if (col0 + u < p.head_dim)
-              *(uint4*)(dst + u) = make_uint4(pack2(T(), o[u], o[u + 1]), pack2(T(), o[u + 2], o[u + 3]),
-                                              pack2(T(), o[u + 4], o[u + 5]), pack2(T(), o[u + 6], o[u + 7]));
+          for (int u = 0; u < 4; ++u)
+            v[u] = make_uint4(pack2(T(), o[8 * u], o[8 * u + 1]), pack2(T(), o[8 * u + 2], o[8 * u + 3]),
+                              pack2(T(), o[8 * u + 4], o[8 * u + 5]), pack2(T(), o[8 * u + 6], o[8 * u + 7]));
+          exchange<1>(v, lane);
+          exchange<2>(v, lane);
+          const uint32_t col = col0 + 8 * (lane & 3);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const uint64_t to = __shfl_sync(0xffffffffu, row_at, (lane & ~3) + u);
+            if (to != ~0ull && col < p.head_dim) *(uint4*)((T*)p.out + to + col) = v[u];
+          }
         }
         __syncwarp();  // TMEM loads are the whole warp's
       }
@@ -632,8 +759,7 @@ cudaError_t launch(const AttnParams& p, uint32_t dtype, cudaStream_t st) {
     cudaFuncAttributes fa{};
     const cudaError_t f = cudaFuncGetAttributes(&fa, attention_tc_kernel<T, HDP>);
     if (f != cudaSuccess) return f;
-    fits.store(kRegsControl + 2 * kRegsSoftmax <= 3 * fa.numRegs && kRegsControl <= fa.numRegs &&
-               fa.numRegs <= kRegsSoftmax);
+    fits.store(fa.numRegs == Shape<HDP>::kRegs);
   }
   if (!fits.load()) return cudaErrorInvalidConfiguration;
   const uint32_t rows = attention_tc_tile_rows(p.group);
@@ -645,7 +771,7 @@ cudaError_t launch(const AttnParams& p, uint32_t dtype, cudaStream_t st) {
       !head_map(&v, p.total_k ? p.v : p.q, dtype, p.total_k ? p.total_k : 1, p.total_k ? p.kv_heads : 1, p.head_dim,
                 p.total_k ? p.ld_v : p.ld_q, 1, kKeyTile))
     return cudaErrorInvalidValue;
-  attention_tc_kernel<T, HDP><<<p.blocks, kThreads, smem, st>>>(p, q, k, v, rows);
+  attention_tc_kernel<T, HDP><<<p.blocks, Shape<HDP>::kThreads, smem, st>>>(p, q, k, v, rows);
   return cudaGetLastError();
 }
 
