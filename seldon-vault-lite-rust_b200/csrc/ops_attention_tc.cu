@@ -4,15 +4,15 @@
 // One persistent CTA per SM walks its segments (rows of one key-value head
 // against a list of 128-key tiles).  A row tile is up to 128 (query, head of the
 // group) rows, so every head of a group reads a key tile once.  Head sizes up to
-// 128: two row tiles share each key tile, one softmax warpgroup each, so that one
-// tile's products run under the other's softmax.  Head sizes up to 256: one row
-// tile with two score buffers, its 128 columns split between the two warpgroups.
-// (Two warpgroups a row tile for the small heads too were measured at 610 us
-// against UNMEASURED for the 8192-token prefix case: 96 registers a thread send
-// the scores through TMEM twice.)
+// 128: two row tiles share each key tile, so that one tile's products run under
+// the other's softmax.  Head sizes up to 256: one row tile with two score
+// buffers.  Two softmax warpgroups share a row tile, 64 of a key tile's columns
+// each: with one of them a scheduler has a single softmax warp for each row tile,
+// whose chains of dependent instructions it cannot fill (622 against UNMEASURED us for
+// the 8192-token prefix case).
 //
 //   S = Q K^T  128 x 128 into TMEM (kind::f16, FP32 accumulators)
-//   softmax    a row (or half of one) per thread: running maximum m and sum l; weights
+//   softmax    half a row per thread: running maximum m and sum l; weights
 //              P = 2^(t - m) rounded to the type over S's own columns.  m
 //              follows the row's maximum only once it is more than 2^8 behind,
 //              so O is rarely rescaled; the weights stay below 2^8.
@@ -28,22 +28,24 @@
 namespace svl {
 namespace {
 
-constexpr int kThreads = 384;  // warpgroup 0: loads, MMAs, checks; 1 and 2: softmax
-constexpr int kRegs = 168;     // of a thread at launch
-constexpr int kRegsControl = 72, kRegsSoftmax = 216;
-static_assert(kRegsControl + 2 * kRegsSoftmax == 3 * kRegs, "registers move inside the launch's own");
+constexpr int kCols = 64;  // score columns of a softmax thread
+// Tensor-memory columns of the weights of keys 16 k ..: each thread's lie over its own scores.
+SVL_DEV uint32_t weights_at(int k) { return k * 16 / kCols * kCols + k * 16 % kCols / 2; }
 
 template <int HDP>
 struct Shape {
   static constexpr int kRowTiles = HDP <= 128 ? 2 : 1;
   static constexpr int kAhead = HDP <= 128 ? 1 : 2;       // score tiles of a row tile in flight
   static constexpr int kSlabs = HDP / kSlabCols;          // of a K or V tile
-  static constexpr int kStages = HDP == 64 ? 12 : HDP == 128 ? 10 : 9;
-  static constexpr int kHalves = 3 - kRowTiles;           // softmax threads of a row
-  static constexpr int kCols = 128 / kHalves, kOutCols = HDP / kHalves;  // score and output columns of one
+  static constexpr int kStages = HDP == 64 ? 11 : 9;
+  static constexpr int kOutCols = HDP / 2;                // output columns of a softmax thread
   static constexpr uint32_t kOutTmem = 256;
-  // Tensor-memory columns of the weights of keys 16 k ..: each thread's lie over its own scores.
-  static SVL_DEV uint32_t weights_at(int k) { return k * 16 / kCols * kCols + k * 16 % kCols / 2; }
+  // warpgroup 0: loads, MMAs, checks; the others: softmax
+  static constexpr int kSoftmax = 2 * kRowTiles, kThreads = 128 * (1 + kSoftmax);
+  static constexpr int kRegs = kRowTiles == 2 ? 96 : 168;  // of a thread at launch: 65536 / kThreads, in eights
+  static constexpr int kRegsControl = kRowTiles == 2 ? 64 : 72;
+  static constexpr int kRegsSoftmax = kRowTiles == 2 ? 104 : 216;
+  static_assert(kRegsControl + kSoftmax * kRegsSoftmax == (1 + kSoftmax) * kRegs, "registers move inside the launch's own");
 };
 
 struct Mailbox {
@@ -59,7 +61,7 @@ struct Smem {
   uint32_t tmem;
   Mailbox mail;
   uint32_t spoiled[2];  // 1 + the CTA's last segment of that parity with non-finite values
-  float shared_row[Shape<HDP>::kHalves == 2 ? 2 : 1][2][Shape<HDP>::kHalves == 2 ? 128 : 1];  // [parity][half]: maxima, sums
+  float shared_row[2][Shape<HDP>::kRowTiles][2][128];  // [parity][row tile][half]: maxima, sums
 };
 static_assert(sizeof(Smem<64>) + 1024 <= kSmemLimit && sizeof(Smem<128>) + 1024 <= kSmemLimit &&
                   sizeof(Smem<256>) + 1024 <= kSmemLimit,
@@ -108,7 +110,7 @@ SVL_DEV void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32
 SVL_DEV void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 template <typename T, int HDP>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
     attention_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap map_q,
                         const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                         const uint32_t tile_rows) {
@@ -130,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&sm.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_ready[i], 4 * Sh::kHalves);
+      mbar_init(&sm.p_ready[i], 8);
       mbar_init(&sm.pv_done[i], 1);
     }
     mbar_init(&sm.check_req, 1);
@@ -152,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t seg0 = p.block_segments[blockIdx.x], seg1 = p.block_segments[blockIdx.x + 1];
 
   if (warp < 4) {
-    setmaxnreg_dec<kRegsControl>();
+    setmaxnreg_dec<Sh::kRegsControl>();
     if (warp == 0 && lane == 0) {
       // ------------------------------------------------------------- loads --
       const uint32_t q_bytes = tile_rows * 128;  // of one slab
@@ -254,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            mma_f16_ts(tmem + Sh::kOutTmem + t * HDP, tmem + buf * 128 + Sh::weights_at(k), b + k * 128, idesc_o,
+            mma_f16_ts(tmem + Sh::kOutTmem + t * HDP, tmem + buf * 128 + weights_at(k), b + k * 128, idesc_o,
                        k ? 1 : accumulate);
           if (release)
             for (int c = 0; c < slabs; ++c) mma_commit(&sm.empty[at.stage + c]);
@@ -402,11 +404,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // -------------------------------------------------------------- softmax --
-    setmaxnreg_inc<kRegsSoftmax>();
+    setmaxnreg_inc<Sh::kRegsSoftmax>();
     const int wg = (warp - 4) >> 2, lg = warp & 3;
-    constexpr int kCols = Sh::kCols;
-    const int t = kTiles == 2 ? wg : 0, half = kTiles == 2 ? 0 : wg;  // row tile, columns
+    const int t = wg >> 1, half = wg & 1;  // row tile, columns
     const int r = lg * 32 + lane;
+    const int pair = 1 + t * 4 + lg;       // the barrier of the two warps of these rows
     const uint32_t lane_addr = tmem + ((uint32_t)(lg * 32) << 16);
     const uint32_t out_addr = lane_addr + Sh::kOutTmem + t * HDP + half * Sh::kOutCols;
     const bool capped = p.cap > 0.0f, biased = p.slopes != nullptr, plain = !capped && !biased;
@@ -453,13 +455,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (see == kSeesNone) continue;
         const int buf = kTiles == 2 ? t : (int)(g & 1);
         const int64_t j0 = (int64_t)entry_tile(e) * kKeyTile + half * kCols;
-        // a lane loads every 32nd key's document, under the wait for the scores
-        int32_t docs[kCols / 32];
-#pragma unroll
-        for (int h = 0; h < kCols / 32; ++h) docs[h] = -1;
+        // a lane loads two keys' documents, under the wait for the scores
+        int32_t docs[2] = {-1, -1};
         if (p.doc_k && see == kSeesSome) {
 #pragma unroll
-          for (int h = 0; h < kCols / 32; ++h)
+          for (int h = 0; h < 2; ++h)
             if (j0 + 32 * h + lane < (int64_t)s.n_k) docs[h] = __ldg(p.doc_k + s.k0 + j0 + 32 * h + lane);
         }
         wait(&sm.s_full[buf], (kTiles == 2 ? g : g >> 1) & 1);
@@ -476,45 +476,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float rise = gap > 0.0f ? slope2 : -slope2;  // direct bias: -slope |gap - c| = rise (c - gap)
         float top = -INFINITY;
         bool small = true;  // every score within the cap's polynomial
-        uint32_t w[kCols];                // a direct tile's scores stay in registers
         if (direct) {
+          float low = INFINITY;
+#pragma unroll 1
+          for (int c0 = 0; c0 < kCols; c0 += 32) {
+            uint32_t w[32];
+            tmem_ld32_nowait(s_addr + c0, w);
+            tmem_ld_wait();
+            tmem_regs_after_wait(w);
+            auto x = [&](int c) { return __uint_as_float(w[c]); };
+            if (biased) {
+              const uint64_t by2 = two(scale2, scale2), rise2 = two(2.0f * rise, 2.0f * rise);
+              uint64_t t2 = two(rise * ((float)c0 - gap), rise * ((float)c0 - gap) + rise);
 #pragma unroll
-          for (int c0 = 0; c0 < kCols; c0 += 32) tmem_ld32_nowait(s_addr + c0, w + c0);
-          tmem_ld_wait();
-#pragma unroll
-          for (int c0 = 0; c0 < kCols; c0 += 32) tmem_regs_after_wait(w + c0);
-          auto x = [&](int c) { return __uint_as_float(w[c]); };
-          if (biased) {
-            const uint64_t by2 = two(scale2, scale2), rise2 = two(8.0f * rise, 8.0f * rise);
-            uint64_t t2[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) t2[i] = two(rise * ((float)(2 * i) - gap), rise * ((float)(2 * i + 1) - gap));
-#pragma unroll
-            for (int c = 0; c < kCols; c += 8)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                apart(fma_two(two(w[c + 2 * i], w[c + 2 * i + 1]), by2, t2[i]), w[c + 2 * i], w[c + 2 * i + 1]);
-                t2[i] = add_two(t2[i], rise2);
+              for (int c = 0; c < 32; c += 2) {
+                apart(fma_two(two(w[c], w[c + 1]), by2, t2), w[c], w[c + 1]);
+                t2 = add_two(t2, rise2);
               }
-          }
-          constexpr int kPart = kCols / 4;
-          float mx[4], low = 0.0f;
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            mx[u] = fmaxf(x(kPart * u), x(kPart * u + 1));
-#pragma unroll
-            for (int c = 2; c < kPart; c += 2) mx[u] = fmax3(mx[u], x(kPart * u + c), x(kPart * u + c + 1));
-          }
-          top = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
-          if (capped) {
-            float mn[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              mn[u] = fminf(x(kPart * u), x(kPart * u + 1));
-#pragma unroll
-              for (int c = 2; c < kPart; c += 2) mn[u] = fmin3(mn[u], x(kPart * u + c), x(kPart * u + c + 1));
             }
-            low = fminf(fmin3(mn[0], mn[1], mn[2]), mn[3]);
+            float mx[2] = {x(0), x(1)};
+#pragma unroll
+            for (int c = 2; c < 32; c += 4) {
+              mx[0] = fmax3(mx[0], x(c), x(c + 1));
+              if (c + 2 < 32) mx[1] = fmax3(mx[1], x(c + 2), x(c + 3));
+            }
+            top = fmax3(top, mx[0], mx[1]);
+            if (capped) {
+              float mn[2] = {x(0), x(1)};
+#pragma unroll
+              for (int c = 2; c < 32; c += 4) {
+                mn[0] = fmin3(mn[0], x(c), x(c + 1));
+                if (c + 2 < 32) mn[1] = fmin3(mn[1], x(c + 2), x(c + 3));
+              }
+              low = fmin3(low, mn[0], mn[1]);
+            }
           }
           if (plain) top *= scale2;
           if (capped) {
@@ -556,9 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t ahead = bits_below((int)max((int64_t)0, min((int64_t)prefix - j, (int64_t)32)));
             if (p.doc_k) {
               // each document of the 32 in turn gives its keys to its rows
-              int32_t d = docs[0];
-#pragma unroll
-              for (int h = 1; h < kCols / 32; ++h) d = c0 == 32 * h ? docs[h] : d;
+              const int32_t d = c0 ? docs[1] : docs[0];
               const uint32_t member = __ballot_sync(0xffffffffu, d >= 0);
               uint32_t own = 0;
               for (uint32_t left = member; left;) {
@@ -588,12 +581,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_st32(s_addr + c0, w);
           tmem_st_wait();
         }
-        if constexpr (Sh::kHalves == 2) {
-          // both halves of a row follow one maximum
-          sm.shared_row[g & 1][half][r] = top;
-          pair_sync(1 + lg);
-          top = fmaxf(top, sm.shared_row[g & 1][half ^ 1][r]);
-        }
+        // both halves of a row follow one maximum
+        sm.shared_row[g & 1][t][half][r] = top;
+        pair_sync(pair);
+        top = fmaxf(top, sm.shared_row[g & 1][t][half ^ 1][r]);
         float factor = 1.0f;
         if (top > m + kBehind || (m == -INFINITY && top > -INFINITY)) {
           factor = m == -INFINITY ? 0.0f : ex2_approx(m - top);
@@ -616,61 +607,73 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float base = m == -INFINITY ? 0.0f : m;
         uint64_t sum[2] = {0, 0};  // pairs of 0.0f
         // 2^(t - m) of 32 columns; `exponents` makes four pairs of t - m from four of scores
-        auto weights = [&](const uint32_t* v, int c0, auto&& exponents) {
-          uint32_t pk[16];
+        auto weights = [&](auto&& exponents) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < kCols; c0 += 32) {
+            uint32_t w[32], pk[16];
+            tmem_ld32_nowait(s_addr + c0, w);
+            tmem_ld_wait();
+            tmem_regs_after_wait(w);
 #pragma unroll
-          for (int u = 0; u < 16; u += 4) {
-            uint64_t y[4];
+            for (int u = 0; u < 16; u += 4) {
+              uint64_t y[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = two(v[2 * (u + i)], v[2 * (u + i) + 1]);
-            exponents(y);
+              for (int i = 0; i < 4; ++i) y[i] = two(w[2 * (u + i)], w[2 * (u + i) + 1]);
+              exponents(y, c0 + 2 * u);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t a, b;
-              apart(y[i], a, b);
-              const float ea = ex2_approx(__uint_as_float(a)), eb = ex2_approx(__uint_as_float(b));
-              sum[i & 1] = add_two(sum[i & 1], two(ea, eb));
-              pk[u + i] = pack2(T(), ea, eb);
+              for (int i = 0; i < 4; ++i) {
+                uint32_t a, b;
+                apart(y[i], a, b);
+                const float ea = ex2_approx(__uint_as_float(a)), eb = ex2_approx(__uint_as_float(b));
+                sum[i & 1] = add_two(sum[i & 1], two(ea, eb));
+                pk[u + i] = pack2(T(), ea, eb);
+              }
             }
+            tmem_st16(s_addr + c0 / 2, pk);  // over what this warp has read of these columns
           }
-          tmem_st16(s_addr + c0 / 2, pk);  // over what this warp has read of these columns
         };
         const uint64_t base2 = two(-base, -base);
         if (!direct) {
-#pragma unroll 1
-          for (int c0 = 0; c0 < kCols; c0 += 32) {
-            uint32_t v[32];
-            tmem_ld32_nowait(s_addr + c0, v);
-            tmem_ld_wait();
-            tmem_regs_after_wait(v);
-            weights(v, c0, [&](uint64_t* y) {
+          weights([&](uint64_t* y, int) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) y[i] = add_two(y[i], base2);
-            });
-          }
-        } else if (capped && small) {
-          const CapOdd odd(p);
-#pragma unroll
-          for (int c0 = 0; c0 < kCols; c0 += 32)
-            weights(w + c0, c0, [&](uint64_t* y) {
+            for (int i = 0; i < 4; ++i) y[i] = add_two(y[i], base2);
+          });
+        } else if (capped) {
+          if (small) {
+            const CapOdd odd(p);
+            weights([&](uint64_t* y, int) {
               uint64_t r[4];
               odd.over(y, r);
 #pragma unroll
               for (int i = 0; i < 4; ++i) y[i] = fma_two(y[i], r[i], base2);
             });
-        } else {
-          if (capped) {
+          } else {
+            weights([&](uint64_t* y, int) {
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) w[c] = __float_as_uint(capped_any(__uint_as_float(w[c]), cap_arg, cap2));
+              for (int i = 0; i < 4; ++i) {
+                uint32_t a, b;
+                apart(y[i], a, b);
+                y[i] = two(capped_any(__uint_as_float(a), cap_arg, cap2) - base, capped_any(__uint_as_float(b), cap_arg, cap2) - base);
+              }
+            });
           }
-          const float by = plain ? scale2 : 1.0f;
-          const uint64_t by2 = two(by, by);
+        } else {
+          // biased: rise (c - gap); plain: no rise
+          const float up = biased ? rise : 0.0f, start = biased ? -rise * gap - base : -base;
+          const uint64_t by2 = two(scale2, scale2), up2 = two(2.0f * up, 2.0f * up);
+          weights([&](uint64_t* y, int c) {
+            if (biased) {
+              uint64_t t2 = two(fmaf(up, (float)c, start), fmaf(up, (float)(c + 1), start));
 #pragma unroll
-          for (int c0 = 0; c0 < kCols; c0 += 32)
-            weights(w + c0, c0, [&](uint64_t* y) {
+              for (int i = 0; i < 4; ++i) {
+                y[i] = fma_two(y[i], by2, t2);
+                t2 = add_two(t2, up2);
+              }
+            } else {
 #pragma unroll
               for (int i = 0; i < 4; ++i) y[i] = fma_two(y[i], by2, base2);
-            });
+            }
+          });
         }
         uint32_t part[2];
         apart(add_two(sum[0], sum[1]), part[0], part[1]);
@@ -682,12 +685,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++g;
       }
       // ------------------------------------------------------------ epilogue --
-      if constexpr (Sh::kHalves == 2) {
+      {
         const int at = g & 1;  // not the last tile's slot, and the next tile writes this one after the barrier
-        sm.shared_row[at][half][r] = l;
-        pair_sync(1 + lg);
-        l += sm.shared_row[at][half ^ 1][r];
-        pair_sync(1 + lg);
+        sm.shared_row[at][t][half][r] = l;
+        pair_sync(pair);
+        l += sm.shared_row[at][t][half ^ 1][r];
+        pair_sync(pair);
       }
       if (started) product_done();
       tc_fence_after();
@@ -769,7 +772,7 @@ cudaError_t launch(const AttnParams& p, uint32_t dtype, cudaStream_t st) {
     cudaFuncAttributes fa{};
     const cudaError_t f = cudaFuncGetAttributes(&fa, attention_tc_kernel<T, HDP>);
     if (f != cudaSuccess) return f;
-    fits.store(fa.numRegs == kRegs);
+    fits.store(fa.numRegs == Shape<HDP>::kRegs);
   }
   if (!fits.load()) return cudaErrorInvalidConfiguration;
   const uint32_t rows = attention_tc_tile_rows(p.group);
@@ -781,7 +784,7 @@ cudaError_t launch(const AttnParams& p, uint32_t dtype, cudaStream_t st) {
       !head_map(&v, p.total_k ? p.v : p.q, dtype, p.total_k ? p.total_k : 1, p.total_k ? p.kv_heads : 1, p.head_dim,
                 p.total_k ? p.ld_v : p.ld_q, 1, kKeyTile))
     return cudaErrorInvalidValue;
-  attention_tc_kernel<T, HDP><<<p.blocks, kThreads, smem, st>>>(p, q, k, v, rows);
+  attention_tc_kernel<T, HDP><<<p.blocks, Shape<HDP>::kThreads, smem, st>>>(p, q, k, v, rows);
   return cudaGetLastError();
 }
 
