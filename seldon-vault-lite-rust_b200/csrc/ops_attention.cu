@@ -27,8 +27,26 @@ inline size_t gen_smem(uint32_t head_dim) {
          3 * kGenRows * 4 + kGenKeys * 4;
 }
 
+// A warp's copy of one operand row into shared memory as FP32, zero behind the
+// head and for rows that are not there.  `wide`: FP32 rows of 16-byte units.
 template <typename T>
-__global__ void __launch_bounds__(kGenThreads) attention_general_kernel(const __grid_constant__ AttnParams p) {
+SVL_DEV void gen_row(float* to, const T* from, uint32_t hd, uint32_t stride, bool there, bool wide, int lane) {
+  if (wide) {
+#pragma unroll
+    for (uint32_t u = 0; u < kAttnMaxHead / 128; ++u) {
+      const uint32_t d = 128 * u + 4 * lane;
+      if (d >= stride) break;
+      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (there && d < hd) x = *(const float4*)(from + d);
+      *(float4*)(to + d) = x;
+    }
+  } else {
+    for (uint32_t d = lane; d < stride; d += 32) to[d] = there && d < hd ? widen(from[d]) : 0.0f;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kGenThreads, 2) attention_general_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ float sm[];
   const uint32_t hd = p.head_dim, stride = gen_stride(hd);
   float* sq = sm;
@@ -43,17 +61,18 @@ __global__ void __launch_bounds__(kGenThreads) attention_general_kernel(const __
   const T* gq = (const T*)p.q;
   const T* gk = (const T*)p.k;
   const T* gv = (const T*)p.v;
+  const bool wide = sizeof(T) == 4 && ((p.ld_q | p.ld_k | p.ld_v | hd) % 4 == 0) &&
+                    ((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) % 16 == 0;
 
   for (uint32_t is = p.block_segments[blockIdx.x]; is < p.block_segments[blockIdx.x + 1]; ++is) {
     const AttnSegment seg = p.segments[is];
     const AttnSeq s = p.seqs[seg.seq];
     __syncthreads();
-    for (uint32_t i = tid; i < kGenRows * stride; i += kGenThreads) {
-      const uint32_t r = i / stride, d = i % stride, row = seg.row0 + r;
-      float x = 0.0f;
-      if (r < seg.rows && d < hd)
-        x = widen(gq[(s.q0 + row / p.group) * p.ld_q + (uint64_t)(seg.kvh * p.group + row % p.group) * hd + d]);
-      sq[i] = x;
+#pragma unroll
+    for (int r = warp; r < kGenRows; r += kGenThreads / 32) {
+      const uint32_t row = seg.row0 + r;
+      gen_row(sq + r * stride, gq + (s.q0 + row / p.group) * p.ld_q + (uint64_t)(seg.kvh * p.group + row % p.group) * hd, hd,
+              stride, r < (int)seg.rows, wide, lane);
     }
     if (tid < kGenRows) {
       s_max[tid] = -INFINITY;
@@ -79,16 +98,17 @@ __global__ void __launch_bounds__(kGenThreads) attention_general_kernel(const __
         const uint32_t j0 = entry_tile(entry) * kKeyTile + sub;
         if (j0 >= s.n_k) break;
         __syncthreads();
-        for (uint32_t i = tid; i < kGenKeys * stride; i += kGenThreads) {
-          const uint32_t j = i / stride, d = i % stride;
-          const bool in = j0 + j < s.n_k && d < hd;
-          const uint64_t row = s.k0 + j0 + j, col = (uint64_t)seg.kvh * hd + d;
-          sk[i] = in ? widen(gk[row * p.ld_k + col]) : 0.0f;
-          sv[i] = in ? widen(gv[row * p.ld_v + col]) : 0.0f;
+#pragma unroll
+        for (int j = warp; j < kGenKeys; j += kGenThreads / 32) {
+          const uint64_t row = s.k0 + j0 + j, col = (uint64_t)seg.kvh * hd;
+          const bool there = j0 + j < s.n_k;
+          gen_row(sk + j * stride, gk + row * p.ld_k + col, hd, stride, there, wide, lane);
+          gen_row(sv + j * stride, gv + row * p.ld_v + col, hd, stride, there, wide, lane);
         }
         if (tid < kGenKeys) s_doc[tid] = p.doc_k && j0 + tid < s.n_k ? p.doc_k[s.k0 + j0 + tid] : 0;
         __syncthreads();
         float dot[2][2] = {};
+#pragma unroll 4
         for (uint32_t d = 0; d < hd; d += 4) {  // the strides' padding is zero
           float4 a[2], b[2];
 #pragma unroll
@@ -140,6 +160,7 @@ __global__ void __launch_bounds__(kGenThreads) attention_general_kernel(const __
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[r][c][e] *= old;
         }
+#pragma unroll 4
         for (int j = 0; j < kGenKeys; ++j) {
           float w[4];
           bool seen[4];
@@ -151,7 +172,7 @@ __global__ void __launch_bounds__(kGenThreads) attention_general_kernel(const __
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const uint32_t d = 128 * c + 4 * lane;
-            if (d >= hd) break;
+            if (d >= hd) continue;
             const float4 x = *(const float4*)(sv + j * stride + d);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
@@ -166,9 +187,10 @@ __global__ void __launch_bounds__(kGenThreads) attention_general_kernel(const __
       }
     }
     __syncthreads();
+#pragma unroll
     for (int r = 0; r < 4; ++r) {
       const uint32_t in_seg = 4 * warp + r, row = seg.row0 + in_seg;
-      if (in_seg >= seg.rows) break;
+      if (in_seg >= seg.rows) continue;
       const float sum = s_sum[in_seg], m = s_max[in_seg];
       const bool empty = m == -INFINITY && sum == 0.0f;
       const float inv = empty ? 0.0f : 1.0f / sum, lse = empty ? -INFINITY : m + logf(sum);
@@ -184,7 +206,7 @@ __global__ void __launch_bounds__(kGenThreads) attention_general_kernel(const __
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t d = 128 * c + 4 * lane + e;
-          if (d >= hd) break;
+          if (d >= hd) continue;
           const float o = empty ? 0.0f : acc[r][c][e] * inv;
           if (seg.slot >= 0) p.part_o[part * hd + d] = o;
           else ((T*)p.out)[token * p.ld_out + (uint64_t)head * hd + d] = narrow<T>(o);
