@@ -13,8 +13,10 @@ namespace {
 // ------------------------------------------------------ the general kernel --
 //
 // One pass over the keys with the running maximum and sum of each row's
-// softmax, in FP32 throughout.
-constexpr int kGenRows = 32, kGenKeys = 32, kGenThreads = 256;
+// softmax, in FP32 throughout.  A block takes 32 rows, or 8 where 32 would leave
+// SMs without a block (one 32-token query of 4 heads of 256: 22 us with 4 blocks,
+// UNMEASURED us with 16).
+constexpr int kGenRows = 32, kGenFewRows = 8, kGenKeys = 32, kGenThreads = 256;
 
 // Row stride of the staged operands in floats: a multiple of 4 whose quarter
 // is odd, so that eight rows' 16-byte reads touch all banks once.
@@ -22,9 +24,8 @@ __host__ __device__ inline uint32_t gen_stride(uint32_t head_dim) {
   const uint32_t quarters = (head_dim + 3) / 4;
   return 4 * (quarters | 1);
 }
-inline size_t gen_smem(uint32_t head_dim) {
-  return (size_t)(kGenRows + 2 * kGenKeys) * gen_stride(head_dim) * 4 + kGenRows * (kGenKeys + 4) * 4 +
-         3 * kGenRows * 4 + kGenKeys * 4;
+inline size_t gen_smem(uint32_t head_dim, int rows) {
+  return (size_t)(rows + 2 * kGenKeys) * gen_stride(head_dim) * 4 + rows * (kGenKeys + 4) * 4 + 3 * rows * 4 + kGenKeys * 4;
 }
 
 // A warp's copy of one operand row into shared memory as FP32, zero behind the
@@ -45,18 +46,18 @@ SVL_DEV void gen_row(float* to, const T* from, uint32_t hd, uint32_t stride, boo
   }
 }
 
-template <typename T>
+template <typename T, int ROWS>
 __global__ void __launch_bounds__(kGenThreads, 2) attention_general_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ float sm[];
   const uint32_t hd = p.head_dim, stride = gen_stride(hd);
   float* sq = sm;
-  float* sk = sq + kGenRows * stride;
+  float* sk = sq + ROWS * stride;
   float* sv = sk + kGenKeys * stride;
   float* sp = sv + kGenKeys * stride;        // scores, then weights; masked: -1
-  float* s_max = sp + kGenRows * (kGenKeys + 4);
-  float* s_sum = s_max + kGenRows;
-  float* s_old = s_sum + kGenRows;           // what the row's earlier sums are worth now
-  int32_t* s_doc = (int32_t*)(s_old + kGenRows);
+  float* s_max = sp + ROWS * (kGenKeys + 4);
+  float* s_sum = s_max + ROWS;
+  float* s_old = s_sum + ROWS;           // what the row's earlier sums are worth now
+  int32_t* s_doc = (int32_t*)(s_old + ROWS);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* gq = (const T*)p.q;
   const T* gk = (const T*)p.k;
@@ -69,27 +70,28 @@ __global__ void __launch_bounds__(kGenThreads, 2) attention_general_kernel(const
     const AttnSeq s = p.seqs[seg.seq];
     __syncthreads();
 #pragma unroll
-    for (int r = warp; r < kGenRows; r += kGenThreads / 32) {
+    for (int r = warp; r < ROWS; r += kGenThreads / 32) {
       const uint32_t row = seg.row0 + r;
       gen_row(sq + r * stride, gq + (s.q0 + row / p.group) * p.ld_q + (uint64_t)(seg.kvh * p.group + row % p.group) * hd, hd,
               stride, r < (int)seg.rows, wide, lane);
     }
-    if (tid < kGenRows) {
+    if (tid < ROWS) {
       s_max[tid] = -INFINITY;
       s_sum[tid] = 0.0f;
     }
-    // this thread's scores: rows 2 ty, 2 ty + 1 x keys tx, tx + 16
-    const int ty = tid >> 4, tx = tid & 15;
-    RowMask mask[2];
-    float slope[2];
+    // this thread's scores: rows M ty .. x keys tx, tx + 32 / M
+    constexpr int M = ROWS == 32 ? 2 : 1, kSpan = kGenKeys / M, kOwn = ROWS / 8;
+    const int ty = tid / kSpan, tx = tid % kSpan;
+    RowMask mask[M];
+    float slope[M];
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      const uint32_t row = seg.row0 + min(2 * ty + a, (int)seg.rows - 1);
+    for (int a = 0; a < M; ++a) {
+      const uint32_t row = seg.row0 + min(M * ty + a, (int)seg.rows - 1);
       mask[a] = row_mask(p, s, row / p.group);
       slope[a] = p.slopes ? p.slopes[seg.kvh * p.group + row % p.group] : 0.0f;
     }
-    // this thread's output: rows 4 warp .. 4 warp + 3, columns 128 c + 4 lane ..
-    float acc[4][4][4] = {};
+    // this thread's output: kOwn rows from kOwn warp on, columns 128 c + 4 lane ..
+    float acc[kOwn][4][4] = {};
 
     for (uint32_t il = seg.list0; il < seg.list1; ++il) {
       const uint32_t entry = p.lists[il];
@@ -107,35 +109,35 @@ __global__ void __launch_bounds__(kGenThreads, 2) attention_general_kernel(const
         }
         if (tid < kGenKeys) s_doc[tid] = p.doc_k && j0 + tid < s.n_k ? p.doc_k[s.k0 + j0 + tid] : 0;
         __syncthreads();
-        float dot[2][2] = {};
+        float dot[M][M] = {};
 #pragma unroll 4
         for (uint32_t d = 0; d < hd; d += 4) {  // the strides' padding is zero
-          float4 a[2], b[2];
+          float4 a[M], b[M];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            a[u] = *(const float4*)(sq + (2 * ty + u) * stride + d);
-            b[u] = *(const float4*)(sk + (tx + 16 * u) * stride + d);
+          for (int u = 0; u < M; ++u) {
+            a[u] = *(const float4*)(sq + (M * ty + u) * stride + d);
+            b[u] = *(const float4*)(sk + (tx + kSpan * u) * stride + d);
           }
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+          for (int u = 0; u < M; ++u)
 #pragma unroll
-            for (int w = 0; w < 2; ++w)
+            for (int w = 0; w < M; ++w)
               dot[u][w] = fmaf(a[u].x, b[w].x, fmaf(a[u].y, b[w].y, fmaf(a[u].z, b[w].z, fmaf(a[u].w, b[w].w, dot[u][w]))));
         }
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < M; ++u)
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const uint32_t j = j0 + tx + 16 * w;
+          for (int w = 0; w < M; ++w) {
+            const uint32_t j = j0 + tx + kSpan * w;
             float t = dot[u][w] * p.scale;
             if (p.cap > 0.0f) t = p.cap * tanhf(t / p.cap);
             if (p.slopes) t -= slope[u] * fabsf((float)(mask[u].place - (int64_t)j));
             // a NaN score is a visible key's own: it has to survive the maximum
-            if (some && !sees(p, mask[u], j, s_doc[tx + 16 * w])) t = -INFINITY;
-            sp[(2 * ty + u) * (kGenKeys + 4) + tx + 16 * w] = t;
+            if (some && !sees(p, mask[u], j, s_doc[tx + kSpan * w])) t = -INFINITY;
+            sp[(M * ty + u) * (kGenKeys + 4) + tx + kSpan * w] = t;
           }
         __syncthreads();
-        for (int r = 4 * warp; r < 4 * warp + 4; ++r) {
+        for (int r = kOwn * warp; r < kOwn * warp + kOwn; ++r) {
           const float t = sp[r * (kGenKeys + 4) + lane];
           const float before = s_max[r], m = fmaxf(before, warp_max(t));
           // rows that have seen nothing keep -inf, and their weights are 0
@@ -153,8 +155,8 @@ __global__ void __launch_bounds__(kGenThreads, 2) attention_general_kernel(const
         }
         __syncwarp();  // a warp's rows are its own from here on
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float old = s_old[4 * warp + r];
+        for (int r = 0; r < kOwn; ++r) {
+          const float old = s_old[kOwn * warp + r];
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -162,11 +164,11 @@ __global__ void __launch_bounds__(kGenThreads, 2) attention_general_kernel(const
         }
 #pragma unroll 4
         for (int j = 0; j < kGenKeys; ++j) {
-          float w[4];
-          bool seen[4];
+          float w[kOwn];
+          bool seen[kOwn];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            w[r] = sp[(4 * warp + r) * (kGenKeys + 4) + j];
+          for (int r = 0; r < kOwn; ++r) {
+            w[r] = sp[(kOwn * warp + r) * (kGenKeys + 4) + j];
             seen[r] = !(w[r] < 0.0f);
           }
 #pragma unroll
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(kGenThreads, 2) attention_general_kernel(const
             if (d >= hd) continue;
             const float4 x = *(const float4*)(sv + j * stride + d);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < kOwn; ++r)
               if (seen[r]) {  // a masked value is not multiplied by zero: it may be NaN
                 acc[r][c][0] = fmaf(w[r], x.x, acc[r][c][0]);
                 acc[r][c][1] = fmaf(w[r], x.y, acc[r][c][1]);
@@ -188,8 +190,8 @@ __global__ void __launch_bounds__(kGenThreads, 2) attention_general_kernel(const
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const uint32_t in_seg = 4 * warp + r, row = seg.row0 + in_seg;
+    for (int r = 0; r < kOwn; ++r) {
+      const uint32_t in_seg = kOwn * warp + r, row = seg.row0 + in_seg;
       if (in_seg >= seg.rows) continue;
       const float sum = s_sum[in_seg], m = s_max[in_seg];
       const bool empty = m == -INFINITY && sum == 0.0f;
@@ -508,13 +510,18 @@ int check_offsets(const uint64_t* cu, uint32_t batch, const char* name, char* er
   return SVL_OK;
 }
 
-template <typename T>
+template <typename T, int ROWS>
 cudaError_t launch_general(const svl::AttnParams& p, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  const cudaError_t e = smem_opt_in(svl::attention_general_kernel<T>, (int)svl::gen_smem(svl::kAttnMaxHead), &done);
+  auto kernel = svl::attention_general_kernel<T, ROWS>;
+  const cudaError_t e = smem_opt_in(kernel, (int)svl::gen_smem(svl::kAttnMaxHead, ROWS), &done);
   if (e != cudaSuccess) return e;
-  svl::attention_general_kernel<T><<<p.blocks, svl::kGenThreads, svl::gen_smem(p.head_dim), st>>>(p);
+  kernel<<<p.blocks, svl::kGenThreads, svl::gen_smem(p.head_dim, ROWS), st>>>(p);
   return cudaGetLastError();
+}
+template <typename T>
+cudaError_t launch_general(const svl::AttnParams& p, cudaStream_t st) {
+  return p.slot_rows == svl::kGenRows ? launch_general<T, svl::kGenRows>(p, st) : launch_general<T, svl::kGenFewRows>(p, st);
 }
 
 template <typename T>
@@ -583,6 +590,11 @@ int svl_attention_plan_create(int device, const svl_attention_config* config, co
         tile_rows = svl::attention_tc_tile_rows(group);
         row_tiles = svl::attention_tc_row_tiles(c.head_dim);
       }
+    } else {
+      uint64_t blocks = 0;
+      for (uint32_t b = 0; b < batch; ++b)
+        blocks += ((cu_q[b + 1] - cu_q[b]) * group + svl::kGenRows - 1) / svl::kGenRows * c.kv_heads;
+      if (blocks < (uint64_t)sms) tile_rows = svl::kGenFewRows;
     }
     const Schedule s = schedule(c, cu_q, cu_k, batch, prefix, doc_q, doc_k, tile_rows, row_tiles, (uint32_t)sms * per_sm);
     svl::AttnParams& p = plan->p;
