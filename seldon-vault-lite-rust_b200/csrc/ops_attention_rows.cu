@@ -7,15 +7,18 @@
 // four warps take every other 128-key tile, 32 keys a warp, and each warp keeps
 // the running maximum, sum and output of its own keys in registers, joined at the
 // end.
-// K and V come by TMA through a ring of 16 KB slabs that one thread keeps full
-// across tiles and segments.  (A ninth warp for it would cut the registers of
-// the others from 255 to 168, the outputs of 32 rows or 256 columns out of them.)
+// K and V come by TMA through a ring of 16 KB slabs that a thread of a third
+// warpgroup keeps full across tiles and segments; its registers go to the teams.
 #include "ops_attention_mma.cuh"
 
 namespace svl {
 namespace {
 
-constexpr int kMmaWarps = 8, kThreads = kMmaWarps * 32, kTeam = kMmaWarps / 2, kKeys = 2;  // 16s of keys a warp
+// Warpgroup 0 loads; 1 and 2 are the teams.
+constexpr int kThreads = 384, kMmaWarps = 8, kTeam = kMmaWarps / 2, kKeys = 2;  // 16s of keys a warp
+constexpr int kRegs = 168;  // of a thread at launch
+constexpr int kRegsLoad = 40, kRegsTeam = 232;
+static_assert(kRegsLoad + 2 * kRegsTeam == 3 * kRegs, "registers move inside the launch's own");
 
 // MT tiles of 16 rows.
 template <int HDP, int MT>
@@ -54,41 +57,7 @@ SVL_DEV void mma(__nv_bfloat16, float* d, const uint32_t* a, uint32_t b0, uint32
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-// The CTA's K and V slabs in the order in which they are used: of each segment's
-// key tiles, K's columns and then V's.
-template <int STAGES>
-struct Feeder {
-  RingPos pos;
-  uint32_t segment, entry, slab = 0, issued = 0;
-  int32_t row = 0, kvh = 0;
-  SVL_DEV Feeder(const AttnParams& p, uint32_t first, uint32_t end) : segment(first), entry(0) { enter(p, end, true); }
-  // Goes to the first key tile of this segment or the next that has one.
-  SVL_DEV void enter(const AttnParams& p, uint32_t end, bool fresh) {
-    for (; segment < end; ++segment, fresh = true) {
-      const AttnSegment& seg = p.segments[segment];
-      if (fresh) entry = seg.list0;
-      if (entry < seg.list1) {
-        kvh = (int32_t)seg.kvh;
-        row = (int32_t)(p.seqs[seg.seq].k0 + (uint64_t)entry_tile(p.lists[entry]) * kKeyTile);
-        return;
-      }
-    }
-  }
-  SVL_DEV void issue(const AttnParams& p, uint32_t end, uint8_t* ring, uint64_t* full, const CUtensorMap* k,
-                     const CUtensorMap* v, uint32_t slabs) {
-    mbar_arrive_expect_tx(&full[pos.stage], kSlabBytes);
-    tma_load_3d(ring + pos.stage * kSlabBytes, slab < slabs ? k : v, &full[pos.stage],
-                (int32_t)(slab < slabs ? slab : slab - slabs) * kSlabCols, kvh, row);
-    ++issued;
-    pos.next(STAGES);
-    if (++slab == 2 * slabs) {
-      slab = 0;
-      ++entry;
-      enter(p, end, false);
-    }
-  }
-};
+SVL_DEV void teams_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // Zeroes the non-finite halves of an operand register.
 template <typename T>
@@ -123,36 +92,56 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_trigger();
   const uint32_t seg0 = p.block_segments[blockIdx.x], seg1 = p.block_segments[blockIdx.x + 1];
 
+  if (warp < 4) {
+    setmaxnreg_dec<kRegsLoad>();
+    if (threadIdx.x == 0) {
+      RingPos at;
+      uint32_t issued = 0;
+      bool ok = true;
+      for (uint32_t is = seg0; ok && is < seg1; ++is) {
+        const uint32_t list0 = p.segments[is].list0, list1 = p.segments[is].list1, kvh = p.segments[is].kvh;
+        const uint64_t k0 = p.seqs[p.segments[is].seq].k0;
+        uint32_t next = list0 < list1 ? p.lists[list0] : 0;
+        for (uint32_t il = list0; ok && il < list1; ++il) {
+          const int32_t row = (int32_t)(k0 + (uint64_t)entry_tile(next) * kKeyTile);
+          if (il + 1 < list1) next = p.lists[il + 1];
+          for (int i = 0; i < 2 * slabs; ++i) {
+            if (!mbar_wait(&sm.empty[at.stage], at.phase ^ 1, p.err)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(&sm.full[at.stage], kSlabBytes);
+            tma_load_3d(sm.ring + at.stage * kSlabBytes, i < slabs ? &map_k : &map_v, &sm.full[at.stage],
+                        (i < slabs ? i : i - slabs) * kSlabCols, (int32_t)kvh, row);
+            ++issued;
+            at.next(kStages);
+          }
+        }
+      }
+      if (!ok) {
+        // copies in flight land before the CTA leaves
+        RingPos back;
+        for (uint32_t i = 0; i < issued; ++i) {
+          if (i + kStages >= issued) mbar_wait(&sm.full[back.stage], back.phase, p.err);
+          back.next(kStages);
+        }
+      }
+    }
+    return;
+  }
+  setmaxnreg_inc<kRegsTeam>();
+  const int tid = threadIdx.x - 128, warp_in = warp - 4;
   const int g = lane >> 2, c2 = (lane & 3) * 2, mi = lane >> 3, mr = lane & 7;
   const bool capped = p.cap > 0.0f, biased = p.slopes != nullptr;
   const float scale2 = p.scale * kLog2e, cap2 = p.cap * kLog2e, cap_arg = capped ? 2.0f * scale2 / p.cap : 0.0f;
   const uint32_t q_at = smem_u32(sm.q) + ((mi & 1) * 8 + mr) * Sm::kRowBytes + (mi >> 1) * 16;
   // this warp's keys of a slab: K by (8 keys, 8 columns) blocks, V by the same transposed
-  const int team = warp / kTeam, key0 = warp % kTeam * 16 * kKeys;
+  const int team = warp_in / kTeam, key0 = warp_in % kTeam * 16 * kKeys;
   const uint32_t k_row = key0 + (mi >> 1) * 8 + mr, v_row = key0 + (mi & 1) * 8 + mr;
   RingPos pos;
-  uint32_t at = 0;     // the CTA's slabs before this segment, then the slab that this warp is at
-  bool dead = false;   // a wait ran out: no more waits, but every step is taken
-  const uint32_t feeds_to = threadIdx.x == 0 ? seg1 : seg0;
-  Feeder<kStages> feeder(p, seg0, feeds_to);
-  // Refills what its team is done with.
-  auto feed = [&]() {
-    while (feeder.segment < feeds_to && mbar_test(&sm.empty[feeder.pos.stage], feeder.pos.phase ^ 1))
-      feeder.issue(p, feeds_to, sm.ring, sm.full, &map_k, &map_v, slabs);
-  };
-  // The first `n` slabs, if need be behind slabs that are still in use.
-  auto feed_up_to = [&](uint32_t n) {
-    while (!dead && feeder.issued < n && feeder.segment < feeds_to) {
-      if (!mbar_wait(&sm.empty[feeder.pos.stage], feeder.pos.phase ^ 1, p.err)) dead = true;
-      else feeder.issue(p, feeds_to, sm.ring, sm.full, &map_k, &map_v, slabs);
-    }
-  };
+  uint32_t slabs0 = 0;  // the CTA's slabs before this segment
+  bool dead = false;    // a wait ran out: no more waits, but every step is taken
   auto wait = [&]() {
-    if (threadIdx.x == 0) {
-      feed();
-      feed_up_to(at + 1);
-    }
-    __syncwarp();
     if (!dead && !mbar_wait(&sm.full[pos.stage], pos.phase, p.err)) dead = true;
     __syncwarp();
   };
@@ -160,14 +149,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.empty[pos.stage]);
     pos.next(kStages);
-    ++at;
   };
 
   for (uint32_t is = seg0; is < seg1; ++is) {
     const AttnSegment seg = p.segments[is];
     const AttnSeq s = p.seqs[seg.seq];
-    __syncthreads();  // the last segment's rows and flags are read
-    for (int i = threadIdx.x; i < MT * 16 * (HDP / 8); i += kMmaWarps * 32) {
+    teams_sync();  // the last segment's rows and flags are read
+    for (int i = tid; i < MT * 16 * (HDP / 8); i += kMmaWarps * 32) {
       const int r = i / (HDP / 8), d = i % (HDP / 8) * 8;
       uint4 w = make_uint4(0, 0, 0, 0);
       const uint32_t row = seg.row0 + r;
@@ -176,10 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             (uint64_t)(seg.kvh * p.group + row % p.group) * p.head_dim + d);
       *(uint4*)(sm.q + r * Sm::kRowBytes + d * 2) = w;
     }
-    if (threadIdx.x == 0) {
-      sm.spoiled = 0;
-      feed();
-    }
+    if (tid == 0) sm.spoiled = 0;
     // this thread's rows: g and g + 8 of each row tile
     RowMask mask[MT][2];
     float slope2[MT][2], m[MT][2], l[MT][2], o[MT][HDP / 8][4];
@@ -199,15 +184,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int d = 0; d < HDP / 8; ++d)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[t][d][e] = 0.0f;
-    __syncthreads();
+    teams_sync();
 
-    const uint32_t slabs0 = at;
+    // the query operand stays in registers where there is room
+    constexpr bool kKeepQ = HDP * MT <= 128;
+    uint32_t qa[kKeepQ ? MT : 1][kKeepQ ? HDP / 16 : 1][4];
+    if constexpr (kKeepQ) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int k = 0; k < HDP / 16; ++k) ldmatrix(qa[t][k], q_at + t * 16 * Sm::kRowBytes + k * 32);
+    }
     uint32_t next = seg.list0 + team < seg.list1 ? p.lists[seg.list0 + team] : 0;
 #pragma unroll 1
     for (uint32_t il = seg.list0 + team; il < seg.list1; il += 2) {
       const uint32_t entry = next;
       if (il + 2 < seg.list1) next = p.lists[il + 2];
-      at = slabs0 + (il - seg.list0) * 2 * slabs;
+      const uint32_t at = slabs0 + (il - seg.list0) * 2 * slabs;
       pos.stage = at % kStages;
       pos.phase = at / kStages & 1;
       const uint32_t j0 = entry_tile(entry) * kKeyTile + key0;
@@ -228,7 +221,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
             uint32_t a[4];
-            ldmatrix(a, q_at + t * 16 * Sm::kRowBytes + (c * 4 + k) * 32);
+            if constexpr (kKeepQ) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) a[i] = qa[t][c * 4 + k][i];
+            } else {
+              ldmatrix(a, q_at + t * 16 * Sm::kRowBytes + (c * 4 + k) * 32);
+            }
 #pragma unroll
             for (int n = 0; n < kKeys; ++n) {
               mma(T(), sc[t][2 * n], a, b[n][0], b[n][1]);
@@ -343,10 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (some && __any_sync(0xffffffffu, found) && lane == 0) atomicOr(&sm.spoiled, 1u);
     }
-    // the other team's last tile, before this warp waits for it
-    at = slabs0 + (seg.list1 - seg.list0) * 2 * slabs;
-    if (threadIdx.x == 0) feed_up_to(at);
-    __syncwarp();
+    slabs0 += (seg.list1 - seg.list0) * 2 * slabs;
     // A row's sum lies over its four lanes; then the warps join in halves: the
     // upper half hands maximum, sum and output over, the lower half adds them.
 #pragma unroll
@@ -358,38 +353,38 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
 #pragma unroll 1
     for (int half = kMmaWarps / 2; half >= 1; half /= 2) {
-      if (warp >= half && warp < 2 * half) {
+      if (warp_in >= half && warp_in < 2 * half) {
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int r = t * 16 + u * 8 + g;
             if (c2 == 0) {
-              sm.join_max[warp - half][r] = m[t][u];
-              sm.join_sum[warp - half][r] = l[t][u];
+              sm.join_max[warp_in - half][r] = m[t][u];
+              sm.join_sum[warp_in - half][r] = l[t][u];
             }
 #pragma unroll
             for (int d = 0; d < HDP / 8; ++d)
-              *(float2*)&sm.join[warp - half][r][d * 8 + c2] = make_float2(o[t][d][2 * u], o[t][d][2 * u + 1]);
+              *(float2*)&sm.join[warp_in - half][r][d * 8 + c2] = make_float2(o[t][d][2 * u], o[t][d][2 * u + 1]);
           }
       }
-      __syncthreads();
-      if (warp < half) {
+      teams_sync();
+      if (warp_in < half) {
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int r = t * 16 + u * 8 + g;
-            const float other = sm.join_max[warp][r], top = fmaxf(m[t][u], other);
+            const float other = sm.join_max[warp_in][r], top = fmaxf(m[t][u], other);
             const float mine = m[t][u] == -INFINITY ? 0.0f : ex2_approx(m[t][u] - top);
             const float theirs = other == -INFINITY ? 0.0f : ex2_approx(other - top);
             // a sum that is NaN with a maximum of -inf (every score NaN) stays
-            const float their_sum = sm.join_sum[warp][r];
+            const float their_sum = sm.join_sum[warp_in][r];
             l[t][u] = (l[t][u] != l[t][u] || their_sum != their_sum) ? NAN : l[t][u] * mine + their_sum * theirs;
             m[t][u] = top;
 #pragma unroll
             for (int d = 0; d < HDP / 8; ++d) {
-              const float2 w = *(const float2*)&sm.join[warp][r][d * 8 + c2];
+              const float2 w = *(const float2*)&sm.join[warp_in][r][d * 8 + c2];
               // nothing is taken from a side without weight: what it holds is 0
               if (mine != 1.0f) o[t][d][2 * u] *= mine, o[t][d][2 * u + 1] *= mine;
               o[t][d][2 * u] = fmaf(w.x, theirs, o[t][d][2 * u]);
@@ -397,9 +392,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
       }
-      __syncthreads();
+      teams_sync();
     }
-    if (warp != 0) continue;
+    if (warp_in != 0) continue;
     const bool spoiled = sm.spoiled != 0;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
@@ -433,14 +428,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
   }
-  if (threadIdx.x == 0 && dead) {
-    // copies in flight land before the CTA leaves
-    RingPos back;
-    for (uint32_t i = 0; i < feeder.issued; ++i) {
-      if (i + kStages >= feeder.issued) mbar_wait(&sm.full[back.stage], back.phase, p.err);
-      back.next(kStages);
-    }
-  }
 }
 
 template <typename T, int HDP, int MT>
@@ -449,6 +436,15 @@ cudaError_t launch(const AttnParams& p, uint32_t dtype, cudaStream_t st) {
   const int smem = (int)sizeof(Smem<HDP, MT>) + 1024;
   const cudaError_t e = smem_opt_in(attention_rows_kernel<T, HDP, MT>, smem, &done);
   if (e != cudaSuccess) return e;
+  // setmaxnreg hands the launch's own registers on: an increase beyond them never ends
+  static std::atomic<int> fits{-1};
+  if (fits.load() < 0) {
+    cudaFuncAttributes fa{};
+    const cudaError_t f = cudaFuncGetAttributes(&fa, attention_rows_kernel<T, HDP, MT>);
+    if (f != cudaSuccess) return f;
+    fits.store(fa.numRegs == kRegs);
+  }
+  if (!fits.load()) return cudaErrorInvalidConfiguration;
   CUtensorMap k, v;
   // without keys there is nothing to load: any valid map will do
   const bool keys = p.total_k > 0;
