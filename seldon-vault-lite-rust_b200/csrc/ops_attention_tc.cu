@@ -109,15 +109,16 @@ SVL_DEV void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32
 
 SVL_DEV void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
-template <typename T, int HDP>
+// FULL: heads of HDP columns, not fewer.
+template <typename T, int HDP, bool FULL>
 __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
     attention_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap map_q,
                         const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                         const uint32_t tile_rows) {
   using Sh = Shape<HDP>;
   constexpr int kTiles = Sh::kRowTiles, kAhead = Sh::kAhead;
-  const int slabs = (p.head_dim + kSlabCols - 1) / kSlabCols;  // of a K or V tile
-  const uint32_t stages = Sh::kStages / slabs * slabs;          // whole tiles: theirs lie in one piece
+  const int slabs = FULL ? HDP / kSlabCols : (p.head_dim + kSlabCols - 1) / kSlabCols;  // of a K or V tile
+  const uint32_t stages = Sh::kStages / slabs, stage_bytes = slabs * kSlabBytes;         // a stage is a tile
   extern __shared__ uint8_t raw[];
   Smem<HDP>& sm = *(Smem<HDP>*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   const int warp = one_of(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -161,17 +162,17 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
       RingPos pos;
       uint32_t n_segs = 0, issued = 0;
       bool ok = true;
-      auto slabs_of = [&](const CUtensorMap* map, uint32_t kvh, int64_t row) {
-        for (int s = 0; ok && s < slabs; ++s) {
-          if (!mbar_wait(&sm.empty[pos.stage], pos.phase ^ 1, p.err)) {
-            ok = false;
-            return;
-          }
-          mbar_arrive_expect_tx(&sm.full[pos.stage], kSlabBytes);
-          tma_load_3d(sm.ring + pos.stage * kSlabBytes, map, &sm.full[pos.stage], s * kSlabCols, (int32_t)kvh, (int32_t)row);
-          ++issued;
-          pos.next(stages);
+      auto load = [&](const CUtensorMap* map, uint32_t kvh, int64_t row) {
+        if (!mbar_wait(&sm.empty[pos.stage], pos.phase ^ 1, p.err)) {
+          ok = false;
+          return;
         }
+        mbar_arrive_expect_tx(&sm.full[pos.stage], stage_bytes);
+        for (int c = 0; c < slabs; ++c)
+          tma_load_3d(sm.ring + pos.stage * stage_bytes + c * kSlabBytes, map, &sm.full[pos.stage], c * kSlabCols,
+                      (int32_t)kvh, (int32_t)row);
+        ++issued;
+        pos.next(stages);
       };
       for (uint32_t is = seg0; ok && is < seg1; ++is) {
         const AttnSegment seg = p.segments[is];
@@ -190,10 +191,10 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
             tma_load_3d(sm.q + (t * Sh::kSlabs + c) * kSlabBytes, &map_q, &sm.q_full, c * kSlabCols,
                         (int32_t)(seg.kvh * p.group), (int32_t)(s.q0 + (seg.row0 + t * tile_rows) / p.group));
         auto key_row = [&](uint32_t j) { return (int64_t)s.k0 + (int64_t)entry_tile(p.lists[seg.list0 + j]) * kKeyTile; };
-        for (uint32_t j = 0; j < (uint32_t)kAhead && j < n; ++j) slabs_of(&map_k, seg.kvh, key_row(j));
+        for (uint32_t j = 0; ok && j < (uint32_t)kAhead && j < n; ++j) load(&map_k, seg.kvh, key_row(j));
         for (uint32_t j = 0; ok && j < n; ++j) {
-          slabs_of(&map_v, seg.kvh, key_row(j));
-          if (j + kAhead < n) slabs_of(&map_k, seg.kvh, key_row(j + kAhead));
+          load(&map_v, seg.kvh, key_row(j));
+          if (ok && j + kAhead < n) load(&map_k, seg.kvh, key_row(j + kAhead));
         }
       }
       if (!ok) {
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
       // that one thread takes alone does not compute in (200 cycles a product).
       constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? (1u << 7 | 1u << 10) : 0u;
       const uint32_t idesc_s = idesc_f16(128, 128, 0) | kType;
-      const int k_steps = (p.head_dim + 15) / 16;
+      const int k_steps = FULL ? HDP / 16 : (p.head_dim + 15) / 16;
       const uint32_t idesc_o = idesc_f16(128, k_steps * 16, 1) | kType;
       // shared-memory descriptors at the first byte; addresses go in in 16s
       const uint64_t q_desc = sdesc(smem_u32(sm.q), 16, 1024, kLayoutSW128);
@@ -226,64 +227,41 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
       auto wait = [&](uint64_t* bar, uint32_t phase) {
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, phase, p.err));
       };
-      // the first use of a tile's slabs waits for them
-      auto arrived = [&](RingPos at) {
-        for (int c = 0; c < slabs; ++c) wait(&sm.full[at.stage + c], at.phase);
-      };
-      auto scores = [&](int t, int buf, RingPos at, bool first, bool release) {
-        if (first) arrived(at);
-        if (!ok) return;
-        tc_fence_after();
-        const uint64_t a = q_desc + t * (Sh::kSlabs * kSlabBytes / 16), b = k_desc + at.stage * (kSlabBytes / 16);
-        if (elect_one()) {
+      // by one thread: S of a row tile against the K tile at `at`; the last row tile gives the K tile back
+      auto scores = [&](int t, int buf, RingPos at, bool release) {
+        const uint64_t a = q_desc + t * (Sh::kSlabs * kSlabBytes / 16), b = k_desc + at.stage * (stage_bytes / 16);
 #pragma unroll
-          for (int k = 0; k < HDP / 16; ++k)
-            if (k < k_steps) {
-              const int step = k / 4 * (kSlabBytes / 16) + k % 4 * 2;
-              mma_f16(tmem + buf * 128, a + step, b + step, idesc_s, k != 0);
-            }
-          if (release)
-            for (int c = 0; c < slabs; ++c) mma_commit(&sm.empty[at.stage + c]);
-          mma_commit(&sm.s_full[buf]);
-        }
-        __syncwarp();
+        for (int k = 0; k < HDP / 16; ++k)
+          if (FULL || k < k_steps) {
+            const int step = k / 4 * (kSlabBytes / 16) + k % 4 * 2;
+            mma_f16(tmem + buf * 128, a + step, b + step, idesc_s, k != 0);
+          }
+        mma_commit(&sm.s_full[buf]);
+        if (release) mma_commit(&sm.empty[at.stage]);
       };
-      auto outputs = [&](int t, int buf, RingPos at, bool first, bool accumulate, bool release) {
-        if (first) arrived(at);
-        if (!ok) return;
-        tc_fence_after();
-        const uint64_t b = v_desc + at.stage * (kSlabBytes / 16);
-        if (elect_one()) {
+      // by one thread: O of a row tile += P V
+      auto outputs = [&](int t, int buf, RingPos at, bool accumulate, bool release) {
+        const uint64_t b = v_desc + at.stage * (stage_bytes / 16);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            mma_f16_ts(tmem + Sh::kOutTmem + t * HDP, tmem + buf * 128 + weights_at(k), b + k * 128, idesc_o,
-                       k ? 1 : accumulate);
-          if (release)
-            for (int c = 0; c < slabs; ++c) mma_commit(&sm.empty[at.stage + c]);
-          mma_commit(&sm.pv_done[buf]);
-        }
-        __syncwarp();
+        for (int k = 0; k < 8; ++k)
+          mma_f16_ts(tmem + Sh::kOutTmem + t * HDP, tmem + buf * 128 + weights_at(k), b + k * 128, idesc_o,
+                     k ? 1 : accumulate);
+        mma_commit(&sm.pv_done[buf]);
+        if (release) mma_commit(&sm.empty[at.stage]);
       };
-      auto q_done = [&]() {
-        if (ok && elect_one()) mma_commit(&sm.q_empty);
-        __syncwarp();
-      };
-      // Asks the check warps for a V tile at `at`, once it is there.
+      // Asks the check warps for the V tile at `at`, which is there.
       bool checking = false;
       auto ask = [&](RingPos at) {
-        arrived(at);
-        if (!ok) return;
-        if (lane == 0) {
+        if (ok && lane == 0) {
           sm.mail = {at.stage | at.phase << 31, n_segs};
           mbar_arrive(&sm.check_req);
         }
         __syncwarp();
-        checking = true;
+        checking = ok;
       };
       auto checked = [&]() {
-        if (!checking) return;
+        if (checking) wait(&sm.check_done, n_checks++ & 1);
         checking = false;
-        wait(&sm.check_done, n_checks++ & 1);
       };
       auto some = [](uint32_t e) { return entry_sees(e, 0) == kSeesSome || entry_sees(e, 1) == kSeesSome; };
       uint32_t g = 0;  // score tiles (one row tile)
@@ -291,57 +269,82 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
         const uint32_t list0 = one_of(p.segments[is].list0), n = one_of(p.segments[is].list1) - list0;
         if (!n) continue;
         const uint32_t* list = p.lists + list0;
-        wait(&sm.q_full, n_segs & 1);
-        ++n_segs;
         // entries come a tile ahead of their use
         uint32_t e = one_of(list[0]), e1 = n > 1 ? one_of(list[1]) : 0;
+        wait(&sm.q_full, n_segs & 1);
+        ++n_segs;
+        wait(&sm.full[pos.stage], pos.phase);
         if constexpr (kTiles == 2) {
           auto sees_any = [&](uint32_t x, int t) { return entry_sees(x, t) != kSeesNone; };
           bool started[2] = {false, false};
-          if (sees_any(e, 0)) scores(0, 0, pos, true, !sees_any(e, 1));
-          if (sees_any(e, 1)) scores(1, 1, pos, !sees_any(e, 0), true);
-          if (n == 1) q_done();
-          pos = ahead(pos, slabs, stages);
+          tc_fence_after();
+          if (ok && elect_one()) {
+            if (sees_any(e, 0)) scores(0, 0, pos, !sees_any(e, 1));
+            if (sees_any(e, 1)) scores(1, 1, pos, true);
+            if (n == 1) mma_commit(&sm.q_empty);
+          }
+          __syncwarp();
+          pos.next(stages);
           for (uint32_t j = 0; ok && j < n; ++j) {
-            uint32_t e2 = j + 2 < n ? list[j + 2] : 0;
-            const RingPos v = pos, k = ahead(pos, slabs, stages);
+            const uint32_t e2 = j + 2 < n ? list[j + 2] : 0;
             const bool more = j + 1 < n;
+            const RingPos v = pos, k = ahead(pos, 1, stages);
+            wait(&sm.full[v.stage], v.phase);
+            if (more) wait(&sm.full[k.stage], k.phase);
             if (some(e)) ask(v);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-              if (sees_any(e, t)) {
+              const bool now = sees_any(e, t), then = more && sees_any(e1, t);
+              if (now) {
                 wait(&sm.p_ready[t], taken[t]++ & 1);
                 checked();
-                outputs(t, t, v, t == 0 || !sees_any(e, 0), started[t], t == 1 || !sees_any(e, 1));
-                started[t] = true;
               }
-              if (more && sees_any(e1, t)) scores(t, t, k, t == 0 || !sees_any(e1, 0), t == 1 || !sees_any(e1, 1));
+              tc_fence_after();
+              if (ok && elect_one()) {
+                if (now) outputs(t, t, v, started[t], t == 1 || !sees_any(e, 1));
+                if (then) scores(t, t, k, t == 1 || !sees_any(e1, 1));
+              }
+              __syncwarp();
+              started[t] |= now;
             }
-            if (j + 2 == n) q_done();
-            pos = ahead(pos, more ? 2 * slabs : slabs, stages);
+            if (j + 2 == n && ok && elect_one()) mma_commit(&sm.q_empty);
+            pos = ahead(pos, more ? 2 : 1, stages);
             e = e1;
             e1 = one_of(e2);
           }
         } else {
-          scores(0, g & 1, pos, true, true);
-          pos = ahead(pos, slabs, stages);
+          tc_fence_after();
+          if (ok && elect_one()) scores(0, g & 1, pos, true);
+          __syncwarp();
+          pos.next(stages);
           if (n > 1) {
-            scores(0, (g + 1) & 1, pos, true, true);
-            pos = ahead(pos, slabs, stages);
+            wait(&sm.full[pos.stage], pos.phase);
+            tc_fence_after();
+            if (ok && elect_one()) scores(0, (g + 1) & 1, pos, true);
+            __syncwarp();
+            pos.next(stages);
           }
-          if (n <= 2) q_done();
+          if (n <= 2 && ok && elect_one()) mma_commit(&sm.q_empty);
           for (uint32_t j = 0; ok && j < n; ++j, ++g) {
-            uint32_t e2 = j + 2 < n ? list[j + 2] : 0;
+            const uint32_t e2 = j + 2 < n ? list[j + 2] : 0;
             const int buf = g & 1;
+            wait(&sm.full[pos.stage], pos.phase);
             if (some(e)) ask(pos);
             wait(&sm.p_ready[buf], taken[buf]++ & 1);
             checked();
-            outputs(0, buf, pos, true, j > 0, true);
-            pos = ahead(pos, slabs, stages);
+            tc_fence_after();
+            if (ok && elect_one()) outputs(0, buf, pos, j > 0, true);
+            __syncwarp();
+            pos.next(stages);
             if (j + 2 < n) {
-              scores(0, buf, pos, true, true);
-              pos = ahead(pos, slabs, stages);
-              if (j + 3 == n) q_done();
+              wait(&sm.full[pos.stage], pos.phase);
+              tc_fence_after();
+              if (ok && elect_one()) {
+                scores(0, buf, pos, true);
+                if (j + 3 == n) mma_commit(&sm.q_empty);
+              }
+              __syncwarp();
+              pos.next(stages);
             }
             e = e1;
             e1 = one_of(e2);
@@ -374,9 +377,9 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
         at.stage = mail.slab & 0x7fffffffu;
         at.phase = mail.slab >> 31;
         bool found = false;
+        mbar_wait(&sm.full[at.stage], at.phase, p.err);  // passed already: orders this thread's reads
         for (int c = 0; c < slabs; ++c) {
-          mbar_wait(&sm.full[at.stage], at.phase, p.err);  // passed already: orders this thread's reads
-          uint4* slab = (uint4*)(sm.ring + at.stage * kSlabBytes);
+          uint4* slab = (uint4*)(sm.ring + at.stage * stage_bytes + c * kSlabBytes);
           uint32_t most[4] = {};
 #pragma unroll 8
           for (int i = 0; i < kSlabBytes / 16 / 64; ++i) {
@@ -395,7 +398,6 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
               slab[i * 64 + tid] = make_uint4(zero(w.x), zero(w.y), zero(w.z), zero(w.w));
             }
           }
-          at.next(stages);
         }
         if (found) sm.spoiled[mail.segment & 1] = mail.segment;
         fence_async_smem();
@@ -760,17 +762,17 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
   }
 }
 
-template <typename T, int HDP>
+template <typename T, int HDP, bool FULL>
 cudaError_t launch(const AttnParams& p, uint32_t dtype, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   const int smem = (int)sizeof(Smem<HDP>) + 1024;
-  const cudaError_t e = smem_opt_in(attention_tc_kernel<T, HDP>, smem, &done);
+  const cudaError_t e = smem_opt_in(attention_tc_kernel<T, HDP, FULL>, smem, &done);
   if (e != cudaSuccess) return e;
   // the registers that setmaxnreg hands over have to come out of the launch's own: an increase beyond them never ends
   static std::atomic<int> fits{-1};
   if (fits.load() < 0) {
     cudaFuncAttributes fa{};
-    const cudaError_t f = cudaFuncGetAttributes(&fa, attention_tc_kernel<T, HDP>);
+    const cudaError_t f = cudaFuncGetAttributes(&fa, attention_tc_kernel<T, HDP, FULL>);
     if (f != cudaSuccess) return f;
     fits.store(fa.numRegs == Shape<HDP>::kRegs);
   }
@@ -784,8 +786,16 @@ cudaError_t launch(const AttnParams& p, uint32_t dtype, cudaStream_t st) {
       !head_map(&v, p.total_k ? p.v : p.q, dtype, p.total_k ? p.total_k : 1, p.total_k ? p.kv_heads : 1, p.head_dim,
                 p.total_k ? p.ld_v : p.ld_q, 1, kKeyTile))
     return cudaErrorInvalidValue;
-  attention_tc_kernel<T, HDP><<<p.blocks, Shape<HDP>::kThreads, smem, st>>>(p, q, k, v, rows);
+  attention_tc_kernel<T, HDP, FULL><<<p.blocks, Shape<HDP>::kThreads, smem, st>>>(p, q, k, v, rows);
   return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch(const AttnParams& p, uint32_t dtype, cudaStream_t st) {
+  const uint32_t hd = p.head_dim;
+  if (hd <= 64) return hd == 64 ? launch<T, 64, true>(p, dtype, st) : launch<T, 64, false>(p, dtype, st);
+  if (hd <= 128) return hd == 128 ? launch<T, 128, true>(p, dtype, st) : launch<T, 128, false>(p, dtype, st);
+  return hd == 256 ? launch<T, 256, true>(p, dtype, st) : launch<T, 256, false>(p, dtype, st);
 }
 
 }  // namespace
@@ -800,10 +810,7 @@ uint32_t attention_tc_tile_rows(uint32_t group) { return 128 / group * group; }
 uint32_t attention_tc_row_tiles(uint32_t head_dim) { return head_dim <= 128 ? 2 : 1; }
 
 cudaError_t attention_tc_launch(const AttnParams& p, uint32_t dtype, cudaStream_t st) {
-  const bool half = dtype == SVL_DTYPE_F16;
-  if (p.head_dim <= 64) return half ? launch<__half, 64>(p, dtype, st) : launch<__nv_bfloat16, 64>(p, dtype, st);
-  if (p.head_dim <= 128) return half ? launch<__half, 128>(p, dtype, st) : launch<__nv_bfloat16, 128>(p, dtype, st);
-  return half ? launch<__half, 256>(p, dtype, st) : launch<__nv_bfloat16, 256>(p, dtype, st);
+  return dtype == SVL_DTYPE_F16 ? launch<__half>(p, dtype, st) : launch<__nv_bfloat16>(p, dtype, st);
 }
 
 }  // namespace svl
