@@ -646,8 +646,8 @@ int svl_attention_plan_create(int device, const svl_attention_config* config, co
     if (c.cap > 0) {
       const double k = (double)c.scale / c.cap;
       double power = (double)c.cap * 1.4426950408889634 * k;
-      for (int i = 0; i < 5; ++i, power *= k * k) p.cap_odd[i] = (float)(power * svl::kTanhOdd[i]);
-      p.cap_limit = (float)std::min(0.5 / k, 3.0e38);
+      for (int i = 0; i < svl::kCapTerms; ++i, power *= k * k) p.cap_odd[i] = (float)(power * svl::kTanhOdd[i]);
+      p.cap_limit = (float)std::min(svl::kTanhLimit / k, 3.0e38);
     }
     p.causal = (int32_t)c.causal;
     p.window = c.window;

@@ -8,6 +8,7 @@ namespace svl {
 
 constexpr uint32_t kKeyTile = 128;    // keys of a tile, counted from the sequence's first key
 constexpr uint32_t kAttnMaxHead = 512;
+constexpr int kCapTerms = 4;          // of the capped score's polynomial
 
 // How a row tile sees a key tile.
 enum : uint32_t { kSeesNone = 0, kSeesAll = 1, kSeesSome = 2 };
@@ -53,7 +54,7 @@ struct AttnParams {
   uint32_t q_heads, kv_heads, group, head_dim;
   uint64_t total_q, total_k;
   float scale, cap;
-  float cap_odd[5], cap_limit;  // capped_small() below
+  float cap_odd[kCapTerms], cap_limit;  // capped_small() of the FP16 / BF16 kernels
   int32_t causal, window;
   // one call's operands
   const void *q, *k, *v;

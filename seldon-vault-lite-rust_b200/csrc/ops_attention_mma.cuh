@@ -14,16 +14,16 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kBehind = 8.0f;  // a maximum follows once it is 2^8 behind (log2 units)
 
 // cap tanh(scale s / cap) of a raw score s in log2 units.  tanh y = y P(y^2) with
-// P of degree 4 fitted to tanh(y) / y for |y| <= 1/2 (relative error 1.3e-8, below
+// P of degree 3 fitted to tanh(y) / y for |y| <= 0.35 (relative error 3.5e-08, below
 // FP32's half step): multiply-adds on the FMA pipe, with the cap and scale in the
 // coefficients.  The general form costs two of the 16 special functions a cycle
 // that the softmax itself needs; a warp takes it when a score of its tile lies
-// behind cap_limit = cap / (2 scale).
-constexpr double kTanhOdd[5] = {0.9999999873738349, -0.33333075792040845, 0.133249069544671, -0.052994230404600086,
-                                0.017151297500408665};
+// behind cap_limit = 0.35 cap / scale.
+constexpr double kTanhOdd[kCapTerms] = {0.9999999659298247, -0.3333243239119307, 0.1329601580300818, -0.04897000350211587};
+constexpr double kTanhLimit = 0.35;
 SVL_DEV float capped_small(const AttnParams& p, float s) {
   const float z = s * s;
-  return s * fmaf(z, fmaf(z, fmaf(z, fmaf(z, p.cap_odd[4], p.cap_odd[3]), p.cap_odd[2]), p.cap_odd[1]), p.cap_odd[0]);
+  return s * fmaf(z, fmaf(z, fmaf(z, p.cap_odd[3], p.cap_odd[2]), p.cap_odd[1]), p.cap_odd[0]);
 }
 
 // Two FP32 values in one register pair, and the packed forms of the FMA pipe.
@@ -56,19 +56,19 @@ SVL_DEV uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
 
 // P of four pairs.
 struct CapOdd {
-  uint64_t k[5];
+  uint64_t k[kCapTerms];
   SVL_DEV CapOdd(const AttnParams& p) {
 #pragma unroll
-    for (int i = 0; i < 5; ++i) k[i] = two(p.cap_odd[i], p.cap_odd[i]);
+    for (int i = 0; i < kCapTerms; ++i) k[i] = two(p.cap_odd[i], p.cap_odd[i]);
   }
   SVL_DEV void over(const uint64_t* s, uint64_t* r) const {
     uint64_t z[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) z[i] = mul_two(s[i], s[i]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = fma_two(z[i], k[4], k[3]);
+    for (int i = 0; i < 4; ++i) r[i] = fma_two(z[i], k[kCapTerms - 1], k[kCapTerms - 2]);
 #pragma unroll
-    for (int j = 2; j >= 0; --j)
+    for (int j = kCapTerms - 3; j >= 0; --j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) r[i] = fma_two(z[i], r[i], k[j]);
   }
