@@ -445,8 +445,8 @@ typedef struct svl_attention_config {
   uint32_t q_heads;              /* a multiple of kv_heads; q_heads / kv_heads <= 65535 */
   uint32_t kv_heads;             /* 1..65535; query head h reads kv head h / (q_heads / kv_heads) */
   uint32_t head_dim;             /* 1..512 */
-  float scale;                   /* finite, > 0 */
-  float cap;                     /* 0 = none; finite, > 0 */
+  float scale;                   /* 1e-30..1e30 */
+  float cap;                     /* 0 = none; 1e-30..1e30, scale / cap at most 1e30 */
   uint32_t causal;               /* 0 or 1 */
   int32_t window;                /* < 0 = none */
   uint32_t reserved[4];          /* zero */
@@ -462,9 +462,9 @@ typedef struct svl_attention_plan svl_attention_plan;
  *   doc_q, doc_k : the document of every packed query / key, or both NULL;
  *                any values, negative = padding; doc_k NULL alone = doc_q, if
  *                cu_k is NULL too
- *   slopes     : q_heads finite values, or NULL
+ *   slopes     : q_heads values in -1e20..1e20, or NULL
  * Errors: SVL_USAGE (bad configuration, offsets that start off 0 or fall,
- * non-finite slopes), SVL_LIMIT_EXCEEDED (2^31 or more keys, or query rows
+ * slopes out of range), SVL_LIMIT_EXCEEDED (2^31 or more keys, or query rows
  * times group, in one sequence; out of memory). */
 int svl_attention_plan_create(int device, const svl_attention_config* config, const uint64_t* cu_q,
                               const uint64_t* cu_k, uint32_t batch, const uint64_t* prefix, const int32_t* doc_q,

@@ -550,8 +550,11 @@ int svl_attention_plan_create(int device, const svl_attention_config* config, co
   if (!c.q_heads || c.q_heads % c.kv_heads || c.q_heads / c.kv_heads > 65535)
     return refuse(SVL_USAGE, "q_heads must be a multiple of kv_heads (at most 65535 times)", err, err_len);
   if (!c.head_dim || c.head_dim > svl::kAttnMaxHead) return refuse(SVL_USAGE, "head_dim is outside 1..=512", err, err_len);
-  if (!(std::isfinite(c.scale) && c.scale > 0)) return refuse(SVL_USAGE, "scale must be finite and positive", err, err_len);
-  if (!(std::isfinite(c.cap) && c.cap >= 0)) return refuse(SVL_USAGE, "cap must be finite and not negative", err, err_len);
+  // within these every product that the kernels form of scale, cap, slope and a
+  // distance below 2^31 is finite in FP32
+  if (!(c.scale >= 1e-30f && c.scale <= 1e30f)) return refuse(SVL_USAGE, "scale is outside 1e-30..=1e30", err, err_len);
+  if (!(c.cap == 0 || (c.cap >= 1e-30f && c.cap <= 1e30f && (double)c.scale / c.cap <= 1e30)))
+    return refuse(SVL_USAGE, "cap is neither 0 nor in 1e-30..=1e30 with scale / cap at most 1e30", err, err_len);
   if (c.causal > 1) return refuse(SVL_USAGE, "causal must be 0 or 1", err, err_len);
   for (uint32_t r : c.reserved)
     if (r) return refuse(SVL_USAGE, "svl_attention_config.reserved must be zero", err, err_len);
@@ -568,7 +571,7 @@ int svl_attention_plan_create(int device, const svl_attention_config* config, co
       return refuse(SVL_LIMIT_EXCEEDED, "a sequence has 2^31 or more keys or query rows", err, err_len);
   if (slopes)
     for (uint32_t h = 0; h < c.q_heads; ++h)
-      if (!std::isfinite(slopes[h])) return refuse(SVL_USAGE, "slopes must be finite", err, err_len);
+      if (!(std::fabs(slopes[h]) <= 1e20f)) return refuse(SVL_USAGE, "slopes are outside -1e20..=1e20", err, err_len);
   return svl::guarded(err, err_len, [&]() -> int {
     std::unique_ptr<svl_attention_plan> plan(new svl_attention_plan());
     svl::DeviceGuard on(device);
@@ -646,8 +649,13 @@ int svl_attention_plan_create(int device, const svl_attention_config* config, co
     if (c.cap > 0) {
       const double k = (double)c.scale / c.cap;
       double power = (double)c.cap * 1.4426950408889634 * k;
-      for (int i = 0; i < svl::kCapTerms; ++i, power *= k * k) p.cap_odd[i] = (float)(power * svl::kTanhOdd[i]);
-      p.cap_limit = (float)std::min(svl::kTanhLimit / k, 3.0e38);
+      // a coefficient that FP32 cannot hold leaves every score to the general form
+      bool held = true;
+      for (int i = 0; i < svl::kCapTerms; ++i, power *= k * k) {
+        held &= std::fabs(power) < 1e37;
+        p.cap_odd[i] = held ? (float)(power * svl::kTanhOdd[i]) : 0.0f;
+      }
+      p.cap_limit = held ? (float)std::min(svl::kTanhLimit / k, 3.0e38) : -1.0f;
     }
     p.causal = (int32_t)c.causal;
     p.window = c.window;

@@ -605,6 +605,89 @@ def test_attention_flat_and_sharp_scores(dtype, by):
     run_attention(dtype, 2, 1, 128, [(150, 150)], by=by, cap=50.0, slopes=True)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_attention_small_caps_and_scales(dtype):
+    """Caps far below and far above the scores, for both kernels of the 16-bit types."""
+    for lens in ([(130, 130)], [(2, 300)]):
+        for cap in (1e-6, 1e-3, 0.3, 1e6, 1e20):
+            run_attention(dtype, 2, 1, 64, lens, cap=cap)
+        run_attention(dtype, 2, 1, 64, lens, scale=1e-20, cap=1e-25)
+        run_attention(dtype, 2, 1, 64, lens, scale=1e-6)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_attention_zero_scores_under_a_tiny_cap(dtype):
+    """Zero queries: every visible key weighs the same, whatever the cap."""
+    t = TYPES[dtype]
+    for n_q in (3, 200):
+        q, k = torch.zeros(n_q, 64, device="cuda", dtype=t), torch.randn(256, 64, device="cuda", generator=gen(2)).to(t)
+        out, lse = torch.empty(n_q, 64, device="cuda", dtype=t), torch.empty(n_q, 1, device="cuda")
+        plan = AttentionPlan(1, 1, 64, [0, n_q], [0, 256], dtype=dtype, scale=1.0, cap=1e-30)
+        ws = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device="cuda")
+        plan.run_device(q.data_ptr(), 64, k.data_ptr(), 64, k.data_ptr(), 64, out.data_ptr(), 64, lse=lse.data_ptr(),
+                        workspace=ws.data_ptr(), workspace_bytes=plan.workspace_bytes, stream=stream())
+        plan.check()
+        # 256 weights of 1 (exact in every type), a sum of 256 products and a division
+        want = k.double().mean(0)
+        assert ((out.double() - want).abs() <= 260 * ULP * k.double().abs().mean(0) + half_step(dtype) * want.abs() +
+                least_half_step(dtype)).all()
+        assert ((lse.double() - math.log(256)).abs() <= 16 * ULP * math.log(256)).all()
+
+
+def test_attention_group_above_a_tile():
+    """130 query heads on one key head: more rows than a tensor-core tile for a single query."""
+    run_attention("bf16", 130, 1, 16, [(1, 40), (3, 200)])
+
+
+FIRST_CALLS = """
+import sys
+sys.path.insert(0, {pkg!r})
+import torch
+from svl.ops import AttentionPlan, AxisRope, Q4Weight
+torch.manual_seed(0)
+n, hd = 200, 64
+qkv = torch.randn(n, 4 * hd, device="cuda").half()
+pos = torch.arange(n, device="cuda", dtype=torch.int32)
+rope, plan = AxisRope(hd, [32]), AttentionPlan(2, 1, hd, [0, n], dtype="f16")
+few = AttentionPlan(2, 1, hd, [0, 1], [0, n], dtype="f16")
+w = Q4Weight.quantize(torch.randn(96, 2 * hd).numpy(), 32)
+ws = torch.empty(max(plan.workspace_bytes, few.workspace_bytes) + 16, dtype=torch.uint8, device="cuda")
+turned, out, last, y = qkv.clone(), qkv.new_empty(n, 2 * hd), qkv.new_empty(1, 2 * hd), qkv.new_empty(n, 96)
+
+def block():
+    s = torch.cuda.current_stream().cuda_stream
+    a, t = qkv.data_ptr(), turned.data_ptr()
+    rope.apply_device("f16", pos.data_ptr(), n, a, 4 * hd, 2, t, 4 * hd, a + 4 * hd, 4 * hd, 1, t + 4 * hd, 4 * hd, stream=s)
+    plan.run_device(t, 4 * hd, t + 4 * hd, 4 * hd, t + 6 * hd, 4 * hd, out.data_ptr(), 2 * hd, workspace=ws.data_ptr(),
+                    workspace_bytes=plan.workspace_bytes, stream=s)
+    few.run_device(t, 4 * hd, t + 4 * hd, 4 * hd, t + 6 * hd, 4 * hd, last.data_ptr(), 2 * hd, workspace=ws.data_ptr(),
+                   workspace_bytes=few.workspace_bytes, stream=s)
+    w.linear_device("f16", out.data_ptr(), 2 * hd, n, y.data_ptr(), 96, stream=s)
+
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):  # the process's first calls
+    block()
+g.replay()
+torch.cuda.synchronize()
+got = [x.clone() for x in (turned, out, last, y)]
+block()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, (turned, out, last, y))) and bool(torch.isfinite(y).all())
+print("same")
+"""
+
+
+def test_first_calls_inside_a_capture():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    pkg = str(Path(__file__).resolve().parent.parent / "seldon-vault-lite-rust_b200")
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(pkg=pkg)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attention_graph(dtype):
     run_attention(dtype, 4, 2, 128, [(60, 60), (1, 900)], fused=False, causal=True, graph=3)

@@ -73,7 +73,8 @@ PLAN = dict(q_heads=4, kv_heads=2, head_dim=64, cu_q=[0, 3, 8])
 @pytest.mark.parametrize("change", [
     dict(dtype="f64"), dict(kv_heads=0), dict(kv_heads=3), dict(q_heads=0), dict(q_heads=1 << 32), dict(head_dim=0),
     dict(head_dim=513), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
-    dict(cap=-1.0), dict(cap=float("nan")), dict(cap=float("inf")), dict(window=-2), dict(window=1 << 31),
+    dict(cap=-1.0), dict(cap=float("nan")), dict(cap=float("inf")), dict(cap=1e-31), dict(cap=2e30), dict(scale=1e-31),
+    dict(scale=2e30), dict(scale=1e3, cap=1e-28), dict(slopes=[1.0, 1.0, 2e20, 1.0]), dict(window=-2), dict(window=1 << 31),
     dict(cu_q=[1, 3, 8]), dict(cu_q=[0, 5, 3]), dict(cu_q=[]), dict(cu_q=[0.0, 1.5, 3.0]), dict(cu_q=[0, -1, 3]),
     dict(cu_k=[0, 3]), dict(cu_k=[0, 9, 8]), dict(prefix=[1]), dict(prefix=[1, -1]), dict(doc_q=[0] * 7),
     dict(doc_k=[0] * 8), dict(doc_q=[0] * 8, cu_k=[0, 1, 2]), dict(doc_q=[1 << 31] * 8), dict(slopes=[1.0] * 3),
