@@ -482,6 +482,8 @@ __global__ void __launch_bounds__(kWarps * 32, ROWS == 1 ? 3 : 2)
 // More columns: the 8 warps take different row blocks of the same span, whose
 // rows of x they share; the blocks of a cluster take a run of the spans each and
 // join their sums through each other's shared memory, in a fixed order.
+// FP32 rows are cut into their BF16 parts once for all warps (each warp for itself:
+// 630 us at 14 rows, 4800 x 26496).
 constexpr int kBlockStages = 3;
 template <typename T, int NT, int GROUP, bool HALF, bool ZEROS>
 __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 1)
@@ -515,18 +517,36 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 1)
   };
   for (int i = 0; i < kBlockStages - 1; ++i) fetch(i, i < count);
 
+  // the span's columns as the product takes them: as they came, or their parts
+  using Tile = XTile<Op>;
+  uint8_t* parts = shared + kBlockStages * kStage;
 #pragma unroll 1
   for (int i = 0; i < count; ++i) {
     const uint8_t* st = shared + i % kBlockStages * kStage;
     copies_wait<kBlockStages - 2>();
     __syncthreads();  // everyone's copies of this stage are there, and everyone is done with the one before
     fetch((i + kBlockStages - 1) % kBlockStages, i + kBlockStages - 1 < count);
+    const uint8_t* tile = st + kWarps * sizeof(Weights<GROUP>);
+    if constexpr (kParts == 3) {
+      for (int v = threadIdx.x; v < rows_here * 32; v += kWarps * 32) {
+        const int row = v >> 5, u = v & 31;  // 4 columns
+        const float4 x4 = *(const float4*)(tile + XTile<T>::unit(row, u) * 16);
+        const float xs[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+          const uint2 w2 = make_uint2(bf16_part(xs[0], part) >> 16 | bf16_part(xs[1], part),
+                                      bf16_part(xs[2], part) >> 16 | bf16_part(xs[3], part));
+          *(uint2*)(parts + Tile::unit(row * 3 + part, u >> 1) * 16 + (u & 1) * 8) = w2;
+        }
+      }
+      __syncthreads();
+      tile = parts;
+    }
     if (!mine) continue;
     multiply_span<Op, GROUP, HALF, ZEROS, NT>(
         acc, ((const Weights<GROUP>*)st)[warp], lane, [&](int t, uint32_t(*b)[8]) {
-          const int c = t * 8 + g, m = min(c / kParts, rows_here - 1);
-          XTile<T>::columns(st + kWarps * sizeof(Weights<GROUP>), XTile<T>::offset(m, q, 0), XTile<T>::offset(m, q, 1),
-                            c % kParts, b);
+          const int c = min(t * 8 + g, rows_here * kParts - 1);
+          Tile::columns(tile, Tile::offset(c, q, 0), Tile::offset(c, q, 1), 0, b);
         });
   }
   copies_wait<0>();
@@ -730,7 +750,8 @@ template <typename T, int NT, int GROUP, bool HALF, bool ZEROS>
 cudaError_t launch_many(const svl::Q4Matrix& m, const Rows& r, cudaStream_t st) {
   constexpr uint32_t kRows = NT * 8 / svl::Operand<T>::kParts, kBlockRows = 16 * svl::kWarps;
   constexpr int ring = svl::kBlockStages * (svl::kWarps * (int)sizeof(svl::Weights<GROUP>) + kRows * svl::XTile<T>::kBytes);
-  constexpr int sums = NT * 8 * (kBlockRows + 4) * 4, smem = ring > sums ? ring : sums;
+  constexpr int all = ring + (svl::Operand<T>::kParts == 3 ? NT * 8 * 256 : 0);
+  constexpr int sums = NT * 8 * (kBlockRows + 4) * 4, smem = all > sums ? all : sums;
   static std::atomic<uint64_t> done{0};
   auto kernel = svl::q4_many_kernel<T, NT, GROUP, HALF, ZEROS>;
   const cudaError_t e = smem_opt_in(kernel, smem, &done);
