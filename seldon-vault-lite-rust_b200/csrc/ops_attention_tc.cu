@@ -8,8 +8,9 @@
 // the other's softmax.  Head sizes up to 256: one row tile with two score
 // buffers.  Two softmax warpgroups share a row tile, 64 of a key tile's columns
 // each: with one of them a scheduler has a single softmax warp for each row tile,
-// whose chains of dependent instructions it cannot fill (622 against UNMEASURED us for
-// the 8192-token prefix case).
+// whose chains of dependent instructions do not fill it (2 sequences of 6000-8192
+// tokens, 16 query and 2 key heads of 128, causal behind a prefix, capped: 597 us
+// with one, 538 with two at the same state of the rest).
 //
 //   S = Q K^T  128 x 128 into TMEM (kind::f16, FP32 accumulators)
 //   softmax    half a row per thread: running maximum m and sum l; weights
@@ -18,11 +19,18 @@
 //              so O is rarely rescaled; the weights stay below 2^8.
 //   O += P V   P from TMEM, V from shared memory
 //
-// K and V come through one ring of 16 KB slabs (128 keys x 64 columns), in
-// the order in which the products take them.  Key tiles that some row sees
+// K and V tiles come through one ring, in slabs of 128 keys x 64 columns, in the
+// order in which the products take them.  Key tiles that some row sees
 // only in part are checked for non-finite values of V, which a weight of zero
 // would turn into NaN: two warps zero them in shared memory before the product,
 // and the epilogue adds them back to the rows that see them.
+//
+// What bounds it: the round from a row tile's scores through its softmax and back
+// to the products.  On that case (440 us, 786 TFLOP/s counted over visible pairs)
+// the products alone, with the softmax only handing over, take 307 us; S reads
+// both operands from shared memory, 8 KB a 64-cycle step, which is all its
+// bandwidth.  Leaving out the cap's polynomial saves 63 us, the maximum 45, the
+// exponentials 26.
 #include "ops_attention_mma.cuh"
 
 namespace svl {
@@ -37,7 +45,7 @@ struct Shape {
   static constexpr int kRowTiles = HDP <= 128 ? 2 : 1;
   static constexpr int kAhead = HDP <= 128 ? 1 : 2;       // score tiles of a row tile in flight
   static constexpr int kSlabs = HDP / kSlabCols;          // of a K or V tile
-  static constexpr int kStages = HDP == 64 ? 11 : 9;
+  static constexpr int kRingSlabs = HDP == 64 ? 11 : 9;
   static constexpr int kOutCols = HDP / 2;                // output columns of a softmax thread
   static constexpr uint32_t kOutTmem = 256;
   // warpgroup 0: loads, MMAs, checks; the others: softmax
@@ -48,15 +56,17 @@ struct Shape {
   static_assert(kRegsControl + kSoftmax * kRegsSoftmax == (1 + kSoftmax) * kRegs, "registers move inside the launch's own");
 };
 
+// What the check warps are asked for: a ring stage with its phase in the top bit
+// (all ones: nothing more), and the segment it belongs to.
 struct Mailbox {
-  uint32_t slab, segment;
+  uint32_t stage, segment;
 };
 
 template <int HDP>
 struct Smem {
   alignas(1024) uint8_t q[Shape<HDP>::kRowTiles * Shape<HDP>::kSlabs * kSlabBytes];
-  uint8_t ring[Shape<HDP>::kStages * kSlabBytes];
-  uint64_t full[Shape<HDP>::kStages], empty[Shape<HDP>::kStages];
+  uint8_t ring[Shape<HDP>::kRingSlabs * kSlabBytes];
+  uint64_t full[Shape<HDP>::kRingSlabs], empty[Shape<HDP>::kRingSlabs];
   uint64_t drained, q_full, q_empty, s_full[2], p_ready[2], pv_done[2], check_req, check_done;
   uint32_t tmem;
   Mailbox mail;
@@ -118,7 +128,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
   using Sh = Shape<HDP>;
   constexpr int kTiles = Sh::kRowTiles, kAhead = Sh::kAhead;
   const int slabs = FULL ? HDP / kSlabCols : (p.head_dim + kSlabCols - 1) / kSlabCols;  // of a K or V tile
-  const uint32_t stages = Sh::kStages / slabs, stage_bytes = slabs * kSlabBytes;         // a stage is a tile
+  const uint32_t stages = Sh::kRingSlabs / slabs, stage_bytes = slabs * kSlabBytes;         // a stage is a tile
   extern __shared__ uint8_t raw[];
   Smem<HDP>& sm = *(Smem<HDP>*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   const int warp = one_of(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -372,10 +382,10 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
           break;
         }
         const Mailbox mail = sm.mail;
-        if (mail.slab == ~0u) break;
+        if (mail.stage == ~0u) break;
         RingPos at;
-        at.stage = mail.slab & 0x7fffffffu;
-        at.phase = mail.slab >> 31;
+        at.stage = mail.stage & 0x7fffffffu;
+        at.phase = mail.stage >> 31;
         bool found = false;
         mbar_wait(&sm.full[at.stage], at.phase, p.err);  // passed already: orders this thread's reads
         for (int c = 0; c < slabs; ++c) {
