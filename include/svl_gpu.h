@@ -418,8 +418,8 @@ void svl_rope_destroy(svl_rope* rope);
  * after another, any int32 values; angles are exact to 2^-32 of a turn however
  * far the position, and products are rounded once to the type.  An output may
  * be its own input (same pointer and ld: in place).  Element alignment
- * suffices; 16-byte aligned rows with an even head are faster.  ld >= heads *
- * head_dim, n_tokens < 2^31 (else SVL_USAGE). */
+ * suffices; 16-byte aligned rows with an even head are faster.  heads *
+ * head_dim <= ld < 2^36, n_tokens < 2^31 (else SVL_USAGE). */
 int svl_rope_apply_device(const svl_rope* rope, int device, uint32_t dtype, const int32_t* d_positions,
                           uint64_t n_tokens, const void* d_q, uint64_t ld_q, uint32_t q_heads, void* d_q_out,
                           uint64_t ld_q_out, const void* d_k, uint64_t ld_k, uint32_t k_heads, void* d_k_out,
@@ -478,7 +478,7 @@ int svl_attention_plan_workspace(const svl_attention_plan* plan, uint64_t* bytes
 
 /* One attention over the plan's batch.  d_lse: q rows x q_heads, or NULL.
  * d_workspace: 16-byte aligned, svl_attention_plan_workspace bytes, contents
- * irrelevant before and after.  ld >= heads * head_dim.  With FP16 / BF16 and
+ * irrelevant before and after.  heads * head_dim <= ld < 2^36.  With FP16 / BF16 and
  * a head_dim that is a multiple of 8, q, k, v and out have to be 16-byte
  * aligned with ld a multiple of 8 (else SVL_USAGE); otherwise element
  * alignment suffices. */
@@ -522,7 +522,8 @@ int svl_q4_read(const svl_q4* weight, uint32_t* n, uint32_t* k, uint32_t* group,
  * tokens, down to a single one); any count below 2^31 works.  Products and
  * sums are FP32 (an F32 x keeps its 24 bits), y is rounded once.  A row with a
  * NaN or infinite value gets non-finite results; the others do not.  Element
- * alignment suffices.  Columns of y behind n are left as they were. */
+ * alignment suffices.  Strides are below 2^36.  Columns of y behind n are left
+ * as they were. */
 int svl_q4_linear_device(const svl_q4* weight, uint32_t dtype, const void* d_x, uint64_t ld_x, uint64_t rows,
                          void* d_y, uint64_t ld_y, void* stream, char* err, size_t err_len);
 

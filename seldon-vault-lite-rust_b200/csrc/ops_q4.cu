@@ -925,6 +925,7 @@ int svl_q4_linear_device(const svl_q4* weight, uint32_t dtype, const void* d_x, 
   if (!d_x || !d_y) return refuse(SVL_USAGE, "null argument", err, err_len);
   const svl::Q4Matrix& m = weight->m;
   if (ld_x < m.k || ld_y < m.n) return refuse(SVL_USAGE, "a row stride is shorter than its row", err, err_len);
+  if (std::max(ld_x, ld_y) >= 1ull << 36) return refuse(SVL_USAGE, "a row stride is 2^36 or more", err, err_len);
   if (((uintptr_t)d_x | (uintptr_t)d_y) & (svl::dtype_size(dtype) - 1))
     return refuse(SVL_USAGE, "misaligned pointer", err, err_len);
   svl::DeviceGuard on(weight->device);

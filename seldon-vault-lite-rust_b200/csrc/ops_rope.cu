@@ -257,6 +257,7 @@ int svl_rope_apply_device(const svl_rope* rope, int device, uint32_t dtype, cons
     if (x->heads > 65535) return refuse(SVL_USAGE, "more than 65535 heads", err, err_len);
     if (x->ld_in < x->heads * hd || x->ld_out < x->heads * hd)
       return refuse(SVL_USAGE, "a row stride is shorter than its heads", err, err_len);
+    if (std::max(x->ld_in, x->ld_out) >= 1ull << 36) return refuse(SVL_USAGE, "a row stride is 2^36 or more", err, err_len);
     if (((uintptr_t)x->in | (uintptr_t)x->out) & mask) return refuse(SVL_USAGE, "misaligned pointer", err, err_len);
     if (x->in == x->out && x->ld_in != x->ld_out)
       return refuse(SVL_USAGE, "in place needs one row stride", err, err_len);

@@ -62,6 +62,15 @@ def test_rope_call_refusals(change):
         rope.apply_device(**{**call, **change})
 
 
+@pytest.mark.parametrize("change", [dict(ld_q=1 << 36), dict(ld_q=-128), dict(ld_q_out=-128), dict(ld_k=1 << 36),
+                                    dict(ld_k_out=-64)])
+def test_rope_refuses_strides_that_wrap(change):
+    call = dict(dtype="f32", positions=FAKE, n_tokens=3, q=FAKE, ld_q=128, q_heads=2, q_out=2 * FAKE, ld_q_out=128,
+                k=FAKE, ld_k=64, k_heads=1, k_out=2 * FAKE, ld_k_out=64)
+    with pytest.raises(errors.UsageError):
+        AxisRope(64, [32]).apply_device(**{**call, **change})
+
+
 def test_rope_of_nothing_needs_no_device():
     AxisRope(64, [32]).apply_device("f32", 0, 0, 0, 0, 2, 0, 0)
     AxisRope(64, [32]).apply_device("f32", 0, 9, 0, 0, 0, 0, 0)
