@@ -249,8 +249,9 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
     const uint32_t n = min((uint32_t)kJoinBatch, j.slots - c0);
     __syncthreads();
     if (tid < (int)n) {
-      const float w = expf(lse[(c0 + tid) * lse_step] - base);  // NaN where a part's rows are
-      weight[tid] = w;
+      // NaN where a part's rows are; -1: a part in which the row sees nothing
+      const float part_lse = lse[(c0 + tid) * lse_step], w = expf(part_lse - base);
+      weight[tid] = part_lse == -INFINITY ? -1.0f : w;
       sum += w;
     }
     __syncthreads();
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
 #pragma unroll 8
       for (uint32_t c = 0; c < n; ++c) {
         const float x = part[(c0 + c) * part_step + d];
-        if (weight[c] != 0.0f) o[u] = fmaf(weight[c], x, o[u]);
+        if (!(weight[c] < 0.0f)) o[u] = fmaf(weight[c], x, o[u]);
       }
     }
   }
@@ -625,6 +626,9 @@ int svl_attention_plan_create(int device, const svl_attention_config* config, co
       return svl::cuda_failure(e, err, err_len);
     }
     e = cudaMemcpy(plan->block, host.data(), host.size(), cudaMemcpyHostToDevice);
+    // a copy from pageable memory may return before it has landed, and a stream
+    // that does not wait for the default one may be the first to read it
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     if (e != cudaSuccess) return svl::cuda_failure(e, err, err_len);
     uint8_t* base = (uint8_t*)plan->block;
     p.err = (uint32_t*)(base + at_err);
@@ -735,6 +739,7 @@ int svl_attention_check(const svl_attention_plan* plan, char* err, size_t err_le
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
   if (e == cudaSuccess) e = cudaMemcpy(&word, plan->p.err, 4, cudaMemcpyDeviceToHost);
   if (e == cudaSuccess && word) e = cudaMemset(plan->p.err, 0, 4);
+  if (e == cudaSuccess && word) e = cudaStreamSynchronize(nullptr);
   if (e != cudaSuccess) return svl::cuda_failure(e, err, err_len);
   std::string message;
   const int rc = svl::status_from_device(word, &message);

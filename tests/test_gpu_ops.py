@@ -302,6 +302,19 @@ def test_linear_refusals():
     assert (y == 5.0).all()
 
 
+@pytest.mark.parametrize("change", [dict(ld_x=-64), dict(ld_x=1 << 36), dict(ld_y=-8), dict(ld_y=1 << 36)])
+def test_linear_refuses_strides_that_wrap(change):
+    codes = torch.zeros(8, 32, dtype=torch.uint8, device="cuda")
+    scales = torch.ones(8, 2, dtype=torch.bfloat16, device="cuda")
+    w = Q4Weight.from_codes(codes.data_ptr(), scales.data_ptr(), 8, 64, 32)
+    x, y = torch.zeros(2, 64, device="cuda"), torch.full((2, 8), 5.0, device="cuda")
+    call = dict(dtype="f32", x=x.data_ptr(), ld_x=64, rows=2, y=y.data_ptr(), ld_y=8)
+    with pytest.raises(errors.UsageError):
+        w.linear_device(**{**call, **change})
+    torch.cuda.synchronize()
+    assert (y == 5.0).all()
+
+
 # -------------------------------------------------------------- attention --
 
 
@@ -569,6 +582,31 @@ def test_attention_value_seen_by_some(dtype, hd, bad):
         assert torch.equal(~torch.isfinite(out.float()), want)
         if not math.isnan(bad):
             assert (out[sees, col].float() == bad).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_value_seen_with_a_vanishing_weight(dtype, rows):
+    """An infinite value reaches the rows that see it although their weight for it is below FP32's range, in the part
+    of a cut axis that holds the largest scores as in any other."""
+    n, hd, col = 9001, 64, 5
+    t = TYPES[dtype]
+    q = torch.full((rows, hd), 8.0, device="cuda", dtype=t)
+    k = torch.zeros(n, hd, device="cuda", dtype=t)
+    k[-1] = 8.0  # a score of 64 * 64 / 8 = 512 against 0
+    v = torch.ones(n, hd, device="cuda", dtype=t)
+    v[3, col] = float("inf")
+    plan = AttentionPlan(1, 1, hd, [0, rows], [0, n], dtype=dtype)
+    assert plan.workspace_bytes > 0
+    ws = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device="cuda")
+    out = torch.empty(rows, hd, device="cuda", dtype=t)
+    plan.run_device(q.data_ptr(), hd, k.data_ptr(), hd, v.data_ptr(), hd, out.data_ptr(), hd, workspace=ws.data_ptr(),
+                    workspace_bytes=plan.workspace_bytes, stream=stream())
+    plan.check()
+    want = torch.zeros(rows, hd, dtype=torch.bool, device="cuda")
+    want[:, col] = True
+    assert torch.equal(~torch.isfinite(out.float()), want)
+    assert (out[~want] == 1.0).all()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
