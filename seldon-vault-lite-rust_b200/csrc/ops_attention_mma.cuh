@@ -17,14 +17,18 @@ constexpr float kBehind = 8.0f;  // a maximum follows once it is 2^8 behind (log
 // P of degree 3 fitted to tanh(y) / y for |y| <= 0.35 (relative error 3.5e-08, below
 // FP32's half step): multiply-adds on the FMA pipe, with the cap and scale in the
 // coefficients.  The general form costs two of the 16 special functions a cycle
-// that the softmax itself needs; a warp takes it when a score of its tile lies
-// behind cap_limit = 0.35 cap / scale.
+// that the softmax itself needs, and its error is of the cap's size.  A score takes
+// it behind cap_limit = 0.35 cap / scale, and by its own size alone: what else the
+// tile holds (masked keys, other sequences, rows behind the tile) decides only
+// whether the warp computes the general form at all.
 constexpr double kTanhOdd[kCapTerms] = {0.9999999659298247, -0.3333243239119307, 0.1329601580300818, -0.04897000350211587};
 constexpr double kTanhLimit = 0.35;
-SVL_DEV float capped_small(const AttnParams& p, float s) {
-  const float z = s * s;
-  return s * fmaf(z, fmaf(z, fmaf(z, p.cap_odd[3], p.cap_odd[2]), p.cap_odd[1]), p.cap_odd[0]);
+SVL_DEV float cap_odd(const AttnParams& p, float s) {
+  const float z = __fmul_rn(s, s);
+  return fmaf(z, fmaf(z, fmaf(z, p.cap_odd[3], p.cap_odd[2]), p.cap_odd[1]), p.cap_odd[0]);
 }
+// (rounded wherever it is used: not one half of a multiply-add)
+SVL_DEV float capped_small(const AttnParams& p, float s) { return __fmul_rn(s, cap_odd(p, s)); }
 
 // Two FP32 values in one register pair, and the packed forms of the FMA pipe.
 SVL_DEV uint64_t two(float lo, float hi) {
@@ -54,7 +58,7 @@ SVL_DEV uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// P of four pairs.
+// cap_odd of four pairs, to the same bits.
 struct CapOdd {
   uint64_t k[kCapTerms];
   SVL_DEV CapOdd(const AttnParams& p) {
@@ -91,8 +95,12 @@ SVL_DEV void capped_small(const AttnParams& p, uint32_t* w) {
 }
 
 // cap - 2 cap / (1 + e^2y); arg = 2 log2(e) scale / cap, cap2 = cap log2(e)
-SVL_DEV float capped_any(float s, float arg, float cap2) {
+SVL_DEV float capped_large(float s, float arg, float cap2) {
   return cap2 - __fdividef(2.0f * cap2, 1.0f + ex2_approx(s * arg));
+}
+// The form that s's own size asks for.
+SVL_DEV float capped_any(const AttnParams& p, float s, float arg, float cap2) {
+  return fabsf(s) <= p.cap_limit ? capped_small(p, s) : capped_large(s, arg, cap2);
 }
 
 SVL_DEV uint32_t pack2(__half, float lo, float hi) { return pack_half2(lo, hi); }

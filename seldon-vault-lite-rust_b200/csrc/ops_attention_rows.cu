@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int n = 0; n < 2 * kKeys; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) sc[t][n][e] = capped_any(sc[t][n][e], cap_arg, cap2);
+              for (int e = 0; e < 4; ++e) sc[t][n][e] = capped_any(p, sc[t][n][e], cap_arg, cap2);
           } else {
 #pragma unroll
             for (int n = 0; n < 2 * kKeys; ++n)

@@ -525,8 +525,8 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
           }
           if (plain) top *= scale2;
           if (capped) {
-            small = !__any_sync(0xffffffffu, fmaxf(top, -low) > p.cap_limit);
-            top = top == -INFINITY ? top : capped_any(top, cap_arg, cap2);  // the cap keeps the order
+            small = !__any_sync(0xffffffffu, live && fmaxf(top, -low) > p.cap_limit);
+            top = top == -INFINITY ? top : capped_large(top, cap_arg, cap2);  // the cap keeps the order
           }
         } else
 #pragma unroll 1
@@ -540,9 +540,9 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
             float most = 0.0f;
 #pragma unroll
             for (int c = 0; c < 32; c += 2) most = fmax3(most, fabsf(x(c)), fabsf(x(c + 1)));
-            if (__any_sync(0xffffffffu, most > p.cap_limit)) {
+            if (__any_sync(0xffffffffu, live && most > p.cap_limit)) {
 #pragma unroll
-              for (int c = 0; c < 32; ++c) w[c] = __float_as_uint(capped_any(x(c), cap_arg, cap2));
+              for (int c = 0; c < 32; ++c) w[c] = __float_as_uint(capped_any(p, x(c), cap_arg, cap2));
             } else {
               capped_small<32>(p, w);
             }
@@ -660,12 +660,17 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
               for (int i = 0; i < 4; ++i) y[i] = fma_two(y[i], r[i], base2);
             });
           } else {
+            // the same bits as above for each score within the limit
+            auto by_size = [&](uint32_t w) {
+              const float s = __uint_as_float(w);
+              return fabsf(s) <= p.cap_limit ? fmaf(s, cap_odd(p, s), -base) : capped_large(s, cap_arg, cap2) - base;
+            };
             weights([&](uint64_t* y, int) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 uint32_t a, b;
                 apart(y[i], a, b);
-                y[i] = two(capped_any(__uint_as_float(a), cap_arg, cap2) - base, capped_any(__uint_as_float(b), cap_arg, cap2) - base);
+                y[i] = two(by_size(a), by_size(b));
               }
             });
           }

@@ -677,6 +677,59 @@ def test_attention_group_above_a_tile():
     run_attention("bf16", 130, 1, 16, [(1, 40), (3, 200)])
 
 
+def attend(plan, q, k, v, hq, hd):
+    out = torch.full((q.shape[0], hq * hd), 5.0, device="cuda", dtype=q.dtype)
+    lse = torch.full((q.shape[0], hq), 5.0, device="cuda")
+    ws = torch.full((plan.workspace_bytes,), 255, dtype=torch.uint8, device="cuda")
+    plan.run_device(q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(),
+                    hq * hd, lse=lse.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=plan.workspace_bytes,
+                    stream=stream())
+    plan.check()
+    return out, lse
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hq,hk,hd", [(3, 1, 64), (5, 1, 128), (12, 1, 256), (6, 2, 72)])
+@pytest.mark.parametrize("n_q,n_k", [(2, 300), (200, 200)])
+@pytest.mark.parametrize("kwargs", [{}, dict(causal=True), dict(slopes=True)], ids=lambda d: ",".join(d) or "plain")
+def test_capped_rows_do_not_depend_on_strangers(dtype, hq, hk, hd, n_q, n_k, kwargs):
+    """The same bits whatever masked keys, the next sequence, other queries of the sequence and an earlier call hold:
+    scores of their own size (about 1, far inside the cap) and of thirty times that and more (far outside)."""
+    g, t = gen(11), TYPES[dtype]
+    pad = 5
+    q = torch.randn(2 * n_q, hq * hd, device="cuda", generator=g).to(t)
+    k = torch.randn(2 * n_k, hk * hd, device="cuda", generator=g).to(t)
+    v = torch.randn(2 * n_k, hk * hd, device="cuda", generator=g).to(t)
+    docs = ([0] * (n_k - pad) + [-1] * pad) * 2
+    slopes = [0.5 ** (h + 1) for h in range(hq)] if kwargs.get("slopes") else None
+    plan = AttentionPlan(hq, hk, hd, [0, n_q, 2 * n_q], [0, n_k, 2 * n_k], dtype=dtype, cap=50.0,
+                         causal=kwargs.get("causal", False), doc_q=[0] * 2 * n_q, doc_k=docs, slopes=slopes)
+    before = AttentionPlan(4, 1, hd, [0, 9600], [0, 128], dtype=dtype)  # whole tiles of rows on every SM
+    fill_q = torch.ones(9600, 4 * hd, device="cuda", dtype=t)
+    fill_k = torch.ones(128, hd, device="cuda", dtype=t)
+
+    def first(rows=n_q, past=0.0, **change):
+        a, b, c = q.clone(), k.clone(), v.clone()
+        hidden = slice(n_k - pad, n_k)
+        if "hidden" in change:
+            for x in (b, c):
+                x[hidden] = x[hidden] * change["hidden"] if math.isfinite(change["hidden"]) else change["hidden"]
+        if "next" in change:
+            for x, n in ((a, n_q), (b, n_k), (c, n_k)):
+                x[n:] *= change["next"]
+        if "last" in change:
+            a[n_q - 1] *= change["last"]
+        attend(before, fill_q * past, fill_k, fill_k, 4, hd)
+        out, lse = attend(plan, a, b, c, hq, hd)
+        return out[:rows].clone(), lse[:rows].clone()
+
+    for rows, change in ((n_q, dict(hidden=30.0)), (n_q, dict(hidden=float("nan"))), (n_q, dict(hidden=float("inf"))),
+                         (n_q, dict(next=30.0)), (n_q, dict(past=100.0)), (n_q - 1, dict(last=30.0))):
+        want, got = first(rows), first(rows, **change)
+        assert torch.isfinite(want[0].float()).all()
+        assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1]), change
+
+
 FIRST_CALLS = """
 import sys
 sys.path.insert(0, {pkg!r})
