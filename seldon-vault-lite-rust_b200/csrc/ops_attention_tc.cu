@@ -57,9 +57,11 @@ struct Shape {
 };
 
 // What the check warps are asked for: a ring stage with its phase in the top bit
-// (all ones: nothing more), and the segment it belongs to.
+// (all ones: nothing more), and for each row tile that sees the key tile its turn:
+// 1 for the first segment of the CTA in which the row tile sees a key, 2 for the
+// next such segment, and so on; 0 if it does not see this key tile.
 struct Mailbox {
-  uint32_t stage, segment;
+  uint32_t stage, turn[2];
 };
 
 template <int HDP>
@@ -70,7 +72,10 @@ struct Smem {
   uint64_t drained, q_full, q_empty, s_full[2], p_ready[2], pv_done[2], check_req, check_done;
   uint32_t tmem;
   Mailbox mail;
-  uint32_t spoiled[2];  // 1 + the CTA's last segment of that parity with non-finite values
+  // [row tile][parity]: its last turn of that parity with non-finite values.  A check
+  // for turn k + 2 follows the products of turn k + 1, which wait for the weights of all
+  // of the row tile's warps, and these have read the flag of turn k by then.
+  uint32_t spoiled[2][2];
   float shared_row[2][Shape<HDP>::kRowTiles][2][128];  // [parity][row tile][half]: maxima, sums
 };
 static_assert(sizeof(Smem<64>) + 1024 <= kSmemLimit && sizeof(Smem<128>) + 1024 <= kSmemLimit &&
@@ -148,7 +153,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
     }
     mbar_init(&sm.check_req, 1);
     mbar_init(&sm.check_done, 64);
-    sm.spoiled[0] = sm.spoiled[1] = 0;
+    for (int i = 0; i < 4; ++i) sm.spoiled[i / 2][i % 2] = 0;
     fence_barrier_init();
     tma_prefetch_desc(&map_q);
     tma_prefetch_desc(&map_k);
@@ -231,7 +236,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
       // V, keys by columns: 64 columns a slab, 16 keys (2 KB) a step
       const uint64_t v_desc = sdesc(smem_u32(sm.ring), kSlabBytes, 1024, kLayoutSW128);
       RingPos pos;
-      uint32_t n_segs = 0, n_checks = 0;
+      uint32_t n_segs = 0, n_checks = 0, turn[2] = {0, 0};
       uint32_t taken[2] = {0, 0};  // p_ready phases
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t phase) {
@@ -259,11 +264,11 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
         mma_commit(&sm.pv_done[buf]);
         if (release) mma_commit(&sm.empty[at.stage]);
       };
-      // Asks the check warps for the V tile at `at`, which is there.
+      // Asks the check warps for the V tile at `at`, which is there, for the turns of the two row tiles.
       bool checking = false;
-      auto ask = [&](RingPos at) {
+      auto ask = [&](RingPos at, uint32_t turn0, uint32_t turn1) {
         if (ok && lane == 0) {
-          sm.mail = {at.stage | at.phase << 31, n_segs};
+          sm.mail = {at.stage | at.phase << 31, {turn0, turn1}};
           mbar_arrive(&sm.check_req);
         }
         __syncwarp();
@@ -301,7 +306,10 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
             const RingPos v = pos, k = ahead(pos, 1, stages);
             wait(&sm.full[v.stage], v.phase);
             if (more) wait(&sm.full[k.stage], k.phase);
-            if (some(e)) ask(v);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              if (sees_any(e, t) && !started[t]) ++turn[t];
+            if (some(e)) ask(v, sees_any(e, 0) ? turn[0] : 0, sees_any(e, 1) ? turn[1] : 0);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
               const bool now = sees_any(e, t), then = more && sees_any(e1, t);
@@ -339,7 +347,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
             const uint32_t e2 = j + 2 < n ? list[j + 2] : 0;
             const int buf = g & 1;
             wait(&sm.full[pos.stage], pos.phase);
-            if (some(e)) ask(pos);
+            if (some(e)) ask(pos, n_segs, 0);  // every key tile of the list is seen: a turn a segment
             wait(&sm.p_ready[buf], taken[buf]++ & 1);
             checked();
             tc_fence_after();
@@ -362,7 +370,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
         }
       }
       if (lane == 0) {
-        sm.mail = {~0u, 0};
+        sm.mail = {~0u, {0, 0}};
         mbar_arrive(&sm.check_req);
         if (!ok) {  // products in flight end before the CTA leaves
           mma_commit(&sm.drained);
@@ -409,7 +417,9 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
             }
           }
         }
-        if (found) sm.spoiled[mail.segment & 1] = mail.segment;
+        if (found)
+          for (int t = 0; t < 2; ++t)
+            if (mail.turn[t]) sm.spoiled[t][mail.turn[t] & 1] = mail.turn[t];
         fence_async_smem();
         mbar_arrive(&sm.check_done);
       }
@@ -427,7 +437,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
     const float scale2 = p.scale * kLog2e;
     const float cap2 = p.cap * kLog2e, cap_arg = capped ? 2.0f * scale2 / p.cap : 0.0f;
     uint32_t g = 0;       // tiles of this warpgroup
-    uint32_t n_segs = 0;
+    uint32_t turn = 0;    // segments in which this row tile has seen a key
     bool dead = false;    // a wait ran out: no more waits, but every step is taken
     auto wait = [&](uint64_t* bar, uint32_t phase) {
       if (!dead && !mbar_wait(bar, phase, p.err)) dead = true;
@@ -443,7 +453,6 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
     for (uint32_t is = seg0; is < seg1; ++is) {
       const AttnSegment seg = p.segments[is];
       const AttnSeq s = p.seqs[seg.seq];
-      if (seg.list1 > seg.list0) ++n_segs;
       if (t * tile_rows >= seg.rows) continue;
       const uint32_t in_seg = t * tile_rows + r;
       const bool live = r < (int)tile_rows && in_seg < seg.rows;
@@ -614,6 +623,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
             tmem_st32(out_addr + c, o);
           }
         }
+        turn += !started;
         started = true;
         __syncwarp();
         const float base = m == -INFINITY ? 0.0f : m;
@@ -711,7 +721,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
       }
       if (started) product_done();
       tc_fence_after();
-      const bool spoiled = started && sm.spoiled[n_segs & 1] == n_segs;
+      const bool spoiled = started && sm.spoiled[t][turn & 1] == turn;
       const bool empty = !started || (m == -INFINITY && l == 0.0f);
       const float inv = empty ? 0.0f : 1.0f / l;
       const float lse = empty ? -INFINITY : kLn2 * ((m == -INFINITY ? 0.0f : m) + log2f(l));

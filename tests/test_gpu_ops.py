@@ -730,6 +730,36 @@ def test_capped_rows_do_not_depend_on_strangers(dtype, hq, hk, hd, n_q, n_k, kwa
         assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1]), change
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("causal,window", [(True, None), (True, 30), (False, 30), (False, None)])
+def test_attention_values_seen_across_many_segments(dtype, hd, causal, window):
+    """Infinite values in several sequences reach exactly the rows that see them where a block walks many segments, of one
+    and of two row tiles in turn, with and without such values."""
+    lens = [300, 40, 150, 7, 260, 129, 64, 20] * 75
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    g, t = gen(hd), TYPES[dtype]
+    x = torch.randn(cu[-1], 4 * hd, device="cuda", generator=g).to(t)
+    q, k, v = x[:, :2 * hd], x[:, 2 * hd:3 * hd], x[:, 3 * hd:]
+    rng = np.random.default_rng(hd)
+    want = np.zeros((cu[-1], 2 * hd), bool)
+    for s, n in enumerate(lens):
+        p = np.arange(n)
+        for _ in range(rng.integers(0, 4)):
+            at, col = int(rng.integers(n)), int(rng.integers(hd))
+            v[int(cu[s]) + at, col] = float("inf")
+            sees = (p >= at) if causal else np.ones(n, bool)
+            if window is not None:
+                sees &= np.abs(p - at) <= window
+            for h in range(2):
+                want[cu[s]:cu[s + 1], h * hd + col] |= sees
+    plan = AttentionPlan(2, 1, hd, cu, dtype=dtype, causal=causal, window=window)
+    for _ in range(3):
+        out, _ = attend(plan, q, k, v, 2, hd)
+        assert torch.equal(torch.isinf(out.float()), torch.from_numpy(want).cuda())
+        assert not torch.isnan(out.float()).any()
+
+
 FIRST_CALLS = """
 import sys
 sys.path.insert(0, {pkg!r})
