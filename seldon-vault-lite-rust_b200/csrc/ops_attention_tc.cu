@@ -671,16 +671,16 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
             });
           } else {
             // the same bits as above for each score within the limit
-            auto by_size = [&](uint32_t w) {
+            auto exponent = [&](uint32_t w) {
               const float s = __uint_as_float(w);
-              return fabsf(s) <= p.cap_limit ? fmaf(s, cap_odd(p, s), -base) : capped_large(s, cap_arg, cap2) - base;
+              return by_size(p, s, fmaf(s, cap_odd(p, s), -base), capped_large(s, cap_arg, cap2) - base);
             };
             weights([&](uint64_t* y, int) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 uint32_t a, b;
                 apart(y[i], a, b);
-                y[i] = two(by_size(a), by_size(b));
+                y[i] = two(exponent(a), exponent(b));
               }
             });
           }
