@@ -434,6 +434,10 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
     const uint32_t lane_addr = tmem + ((uint32_t)(lg * 32) << 16);
     const uint32_t out_addr = lane_addr + Sh::kOutTmem + t * HDP + half * Sh::kOutCols;
     const bool capped = p.cap > 0.0f, biased = p.slopes != nullptr, plain = !capped && !biased;
+    // capped_large is off by up to 2^-20 of the cap, and a weight must stay below
+    // 2^16 (FP16): from the largest raw score on (below) only with caps that leave
+    // that error under 2^1; higher ones take the maximum of the transformed scores
+    const bool mild_cap = p.cap <= 1e6f;
     const float scale2 = p.scale * kLog2e;
     const float cap2 = p.cap * kLog2e, cap_arg = capped ? 2.0f * scale2 / p.cap : 0.0f;
     uint32_t g = 0;       // tiles of this warpgroup
@@ -493,7 +497,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
         // back to TMEM.
         const float gap = (float)(mask.place - j0);
         const bool apart_from = gap >= (float)(kCols - 1) || gap <= 0.0f;
-        const bool direct = see == kSeesAll && (plain || (capped != biased && (capped || __all_sync(0xffffffffu, apart_from))));
+        const bool direct = see == kSeesAll && (plain || (capped != biased && (capped ? mild_cap : __all_sync(0xffffffffu, apart_from))));
         const float rise = gap > 0.0f ? slope2 : -slope2;  // direct bias: -slope |gap - c| = rise (c - gap)
         float top = -INFINITY;
         bool small = true;  // every score within the cap's polynomial
@@ -535,7 +539,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
           if (plain) top *= scale2;
           if (capped) {
             small = !__any_sync(0xffffffffu, live && fmaxf(top, -low) > p.cap_limit);
-            top = top == -INFINITY ? top : capped_large(top, cap_arg, cap2);  // the cap keeps the order
+            top = top == -INFINITY ? top : capped_any(p, top, cap_arg, cap2);  // the cap keeps the order
           }
         } else
 #pragma unroll 1

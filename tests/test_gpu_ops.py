@@ -760,6 +760,46 @@ def test_attention_values_seen_across_many_segments(dtype, hd, causal, window):
         assert not torch.isnan(out.float()).any()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("cap", [1e5, 1e7, 1e8, 1e9, 1e10, 1e12])
+@pytest.mark.parametrize("n_q,n_k,hd", [(256, 256, 64), (256, 512, 128), (130, 256, 256), (2, 512, 128)])
+def test_attention_caps_far_above_the_scores(dtype, cap, n_q, n_k, hd):
+    """A cap far above every score changes nothing: cap tanh(t / cap) = t (1 - (t / cap)^2 / 3), scores here lie below
+    200, and (200 / 1e5)^2 / 3 is 1.4e-6 of t, at most 2.7e-4 in a score."""
+    g, t = gen(7), TYPES[dtype]
+    q = (torch.randn(n_q, hd, device="cuda", generator=g) * 6).to(t)
+    k = (torch.randn(n_k, hd, device="cuda", generator=g) * 6).to(t)
+    v = torch.randn(n_k, hd, device="cuda", generator=g).to(t)
+    out, lse = attend(AttentionPlan(1, 1, hd, [0, n_q], [0, n_k], dtype=dtype, cap=cap), q, k, v, 1, hd)
+    c = dict(dtype=dtype, scale=hd ** -0.5, cap=0.0)
+    qs, ks, vs = (x.cpu().double().numpy() for x in (q, k, v))
+    seen, gap = visible(dict(causal=False, window=None), n_q, n_k, 0, None, None)
+    want, want_lse, tol, tol_lse = attention_reference(c, qs, ks, vs, seen, gap, 0.0)
+    most = np.abs(c["scale"] * qs @ ks.T).max()
+    assert most < 200
+    moved = most ** 3 / (3 * cap ** 2)  # of a score; a weight by twice that, out by twice that of the magnitudes
+    # FP32's own score under a cap: 8 units of the score for tanh, where the general kernel's quotient t / cap rounds
+    score = moved + 8 * ULP * most
+    assert (np.abs(out.cpu().double().numpy() - want) <= tol + 4 * score * np.abs(vs).max()).all()
+    assert (np.abs(lse[:, 0].cpu().double().numpy() - want_lse) <= tol_lse + score).all()
+
+
+@pytest.mark.parametrize("dtype,by", [("f32", 3e4), ("bf16", 3e4), ("f16", 200.0)])
+@pytest.mark.parametrize("n_q,n_k,hd", [(256, 256, 64), (256, 512, 128), (130, 256, 256), (2, 512, 128)])
+@pytest.mark.parametrize("of_scores", [1e-3, 0.1, 1.0, 10.0])
+def test_attention_large_caps_reached(dtype, by, n_q, n_k, hd, of_scores):
+    """Scores of 2e6 to 1e10 and caps of that size: a weighted mean of ones is one."""
+    g, t = gen(9), TYPES[dtype]
+    q = (torch.randn(n_q, hd, device="cuda", generator=g) * by).to(t)
+    k = (torch.randn(n_k, hd, device="cuda", generator=g) * by).to(t)
+    v = torch.ones(n_k, hd, device="cuda", dtype=t)
+    plan = AttentionPlan(1, 1, hd, [0, n_q], [0, n_k], dtype=dtype, scale=1.0, cap=of_scores * by * by * hd ** 0.5)
+    out, lse = attend(plan, q, k, v, 1, hd)
+    # weights rounded to the type before and not in their sum, n additions each, the result rounded
+    tol = 2 * half_step(dtype) + 2 * (n_k + 4) * ULP
+    assert ((out.double() - 1).abs() <= tol).all() and torch.isfinite(lse).all()
+
+
 FIRST_CALLS = """
 import sys
 sys.path.insert(0, {pkg!r})
