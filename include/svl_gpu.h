@@ -418,7 +418,7 @@ void svl_rope_destroy(svl_rope* rope);
  * after another, any int32 values; angles are exact to 2^-32 of a turn however
  * far the position, and products are rounded once to the type.  An output may
  * be its own input (same pointer and ld: in place).  Element alignment
- * suffices; 16-byte aligned rows with an even head are faster.  heads *
+ * suffices (4 bytes for the positions; else SVL_USAGE); 16-byte aligned rows with an even head are faster.  heads *
  * head_dim <= ld < 2^36, n_tokens < 2^31 (else SVL_USAGE). */
 int svl_rope_apply_device(const svl_rope* rope, int device, uint32_t dtype, const int32_t* d_positions,
                           uint64_t n_tokens, const void* d_q, uint64_t ld_q, uint32_t q_heads, void* d_q_out,

@@ -261,6 +261,7 @@ int svl_rope_apply_device(const svl_rope* rope, int device, uint32_t dtype, cons
     if (((uintptr_t)x->in | (uintptr_t)x->out) & mask) return refuse(SVL_USAGE, "misaligned pointer", err, err_len);
     if (x->in == x->out && x->ld_in != x->ld_out)
       return refuse(SVL_USAGE, "in place needs one row stride", err, err_len);
+    if ((uintptr_t)d_positions & 3) return refuse(SVL_USAGE, "misaligned pointer", err, err_len);
   }
   if (!n_tokens || (!q_heads && !k_heads)) return SVL_OK;
   svl::DeviceGuard on(device);

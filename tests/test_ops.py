@@ -71,6 +71,14 @@ def test_rope_refuses_strides_that_wrap(change):
         AxisRope(64, [32]).apply_device(**{**call, **change})
 
 
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_rope_refuses_misaligned_positions(offset):
+    call = dict(dtype="bf16", positions=FAKE + offset, n_tokens=4, q=FAKE, ld_q=128, q_heads=2, q_out=2 * FAKE,
+                ld_q_out=128)
+    with pytest.raises(errors.UsageError):
+        AxisRope(64, [32]).apply_device(**call)
+
+
 def test_rope_of_nothing_needs_no_device():
     AxisRope(64, [32]).apply_device("f32", 0, 0, 0, 0, 2, 0, 0)
     AxisRope(64, [32]).apply_device("f32", 0, 9, 0, 0, 0, 0, 0)
