@@ -498,7 +498,8 @@ typedef struct svl_q4 svl_q4;
 /* From existing codes, in host or in device memory (work that writes them has
  * to be complete); copied into the handle's own layout; synchronous.
  *   codes  : n x k/2 bytes, column 2c in the low half of byte c
- *   scales : n x k/group of scale_dtype (SVL_DTYPE_F16 or SVL_DTYPE_BF16)
+ *   scales : n x k/group of scale_dtype (SVL_DTYPE_F16 or SVL_DTYPE_BF16); 2-byte
+ *            aligned where they are in device memory (else SVL_USAGE)
  *   zeros  : n x k/group bytes (the low four bits), or NULL (8 for all) */
 int svl_q4_create(int device, const uint8_t* codes, const void* scales, uint32_t scale_dtype, const uint8_t* zeros,
                   uint32_t n, uint32_t k, uint32_t group, svl_q4** out, char* err, size_t err_len);

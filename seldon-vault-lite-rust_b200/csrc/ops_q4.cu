@@ -691,13 +691,17 @@ int q4_reserve(svl_q4* w, int device, uint32_t n, uint32_t k, uint32_t group, ui
 }
 
 // Device memory for `bytes`, or `src` itself where it is this device's already.
-cudaError_t on_device(const void* src, size_t bytes, int device, svl::Freed& held, const void** out) {
+bool is_on_device(const void* src, int device) {
   cudaPointerAttributes at{};
-  if (cudaPointerGetAttributes(&at, src) == cudaSuccess && at.type == cudaMemoryTypeDevice && at.device == device) {
+  if (cudaPointerGetAttributes(&at, src) == cudaSuccess) return at.type == cudaMemoryTypeDevice && at.device == device;
+  cudaGetLastError();
+  return false;
+}
+cudaError_t on_device(const void* src, size_t bytes, int device, svl::Freed& held, const void** out) {
+  if (is_on_device(src, device)) {
     *out = src;
     return cudaSuccess;
   }
-  cudaGetLastError();
   cudaError_t e = cudaMalloc(&held.p, bytes);
   if (e == cudaSuccess) e = cudaMemcpy(held.p, src, bytes, cudaMemcpyDefault);
   *out = held.p;
@@ -828,6 +832,8 @@ int svl_q4_create(int device, const uint8_t* codes, const void* scales, uint32_t
     std::unique_ptr<svl_q4> w(new svl_q4());
     svl::DeviceGuard on(device);
     if (on.status != cudaSuccess) return svl::cuda_failure(on.status, err, err_len);
+    // read in place as 16-bit values; host memory is copied, from any address
+    if ((uintptr_t)scales & 1 && is_on_device(scales, device)) return refuse(SVL_USAGE, "misaligned pointer", err, err_len);
     const int rc = q4_reserve(w.get(), device, n, k, group, scale_dtype, zeros != nullptr, err, err_len);
     if (rc) return rc;
     svl::Freed held[3];

@@ -232,6 +232,24 @@ def test_q4_read_returns_what_was_given():
         assert np.array_equal(zz, z.cpu().numpy() if zeros else np.full_like(zz, 8))
 
 
+def test_q4_create_misaligned_scales():
+    """Scales at an odd address: refused in device memory, which is read in place; copied from host memory."""
+    n, k, group = 24, 128, 32
+    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, generator=torch.Generator().manual_seed(0))
+    scales = (torch.rand(n, k // group, generator=torch.Generator().manual_seed(1)) + 0.5).to(torch.float16)
+    odd = torch.zeros(2 * scales.numel() + 1, dtype=torch.uint8)
+    odd[1:] = scales.reshape(-1).view(torch.uint8)
+    assert odd.data_ptr() % 2 == 0
+    on_gpu, c = odd.cuda(), codes.cuda()
+    with pytest.raises(errors.UsageError):
+        Q4Weight.from_codes(c.data_ptr(), on_gpu.data_ptr() + 1, n, k, group, scale_dtype="f16")
+    w = Q4Weight.from_codes(c.data_ptr(), odd.data_ptr() + 1, n, k, group, scale_dtype="f16")
+    assert np.array_equal(w.read()[1], scales.view(torch.int16).numpy().view(np.uint16))
+    # the same bytes, aligned
+    w = Q4Weight.from_codes(c.data_ptr(), on_gpu[1:].clone().data_ptr(), n, k, group, scale_dtype="f16")
+    assert np.array_equal(w.read()[1], scales.view(torch.int16).numpy().view(np.uint16))
+
+
 def as_bf16(bits):
     return (bits.astype(np.uint32) << 16).view(np.float32).astype(np.float64)
 
