@@ -366,11 +366,14 @@ int svl_search_noalloc(const float* d_rows, const uint64_t* d_chunk_ids, uint64_
  * elements and holds its heads one after another, as the fused q, k, v rows
  * of a projection do.  Every pointer belongs to the device of the handle (or
  * of the `device` argument), whatever the calling thread's current device is,
- * which stays as it was.  The *_device calls and the frees of the handles
- * follow `stream` (NULL = the legacy default stream): they return once
- * queued, allocate nothing and never wait, so they may be captured into a
- * CUDA graph; a captured call keeps referring to the handle, which has to
- * outlive the graph.  A handle is never changed by a call, so threads,
+ * which stays as it was.  The *_device calls follow `stream` (NULL = the
+ * legacy default stream): they return once queued, allocate nothing and never
+ * wait, so they may be captured into a CUDA graph; a captured call keeps
+ * referring to the handle, which has to outlive the graph, and a queued one
+ * has to be over before its handle is destroyed.  Destroying a handle frees its
+ * memory at once and may wait for the device; it may happen while a capture
+ * is open, on any thread.  Creating one allocates, copies and waits, and is not
+ * for an open capture.  A handle is never changed by a call, so threads,
  * streams and graphs may share it; outputs and workspaces are the caller's
  * and must not be shared by calls that may overlap.  Outputs must not overlap
  * inputs except where stated.  NULL pointers are accepted where nothing is

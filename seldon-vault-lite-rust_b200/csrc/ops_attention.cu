@@ -292,11 +292,7 @@ struct svl_attention_plan {
   uint32_t max_join_rows = 0;
   uint64_t workspace = 0;
   void* block = nullptr;
-  ~svl_attention_plan() {
-    if (!block) return;
-    svl::DeviceGuard on(device);
-    cudaFree(block);
-  }
+  ~svl_attention_plan() { svl::free_block(device, block); }
 };
 
 using svl::refuse;

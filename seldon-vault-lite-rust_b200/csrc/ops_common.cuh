@@ -35,6 +35,18 @@ struct DeviceGuard {
   DeviceGuard& operator=(const DeviceGuard&) = delete;
 };
 
+// Frees a handle's memory.  cudaFree inside another stream's capture is refused and
+// breaks that capture unless the thread says that it may happen there; a handle can go at
+// any time, with its owner's last reference.
+inline void free_block(int device, void* block) {
+  if (!block) return;
+  DeviceGuard on(device);
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  const bool swapped = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+  cudaFree(block);
+  if (swapped) cudaThreadExchangeStreamCaptureMode(&mode);
+}
+
 inline int refuse(int status, const std::string& message, char* err, size_t err_len) {
   set_err(err, err_len, message);
   return status;

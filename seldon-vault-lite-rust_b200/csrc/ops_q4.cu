@@ -646,11 +646,7 @@ struct svl_q4 {
   svl::Q4Matrix m{};
   int device = -1;
   void* block = nullptr;  // codes, scales and zeros
-  ~svl_q4() {
-    if (!block) return;
-    svl::DeviceGuard on(device);
-    cudaFree(block);
-  }
+  ~svl_q4() { svl::free_block(device, block); }
   size_t code_bytes() const { return (size_t)m.n * (m.k / 2); }
   size_t group_count() const { return (size_t)m.n * (m.k / m.group); }
 };

@@ -13,7 +13,9 @@ passed as addresses (``tensor.data_ptr()``) with row strides in elements; calls
 queue on ``stream`` (a ``cudaStream_t`` as an int, 0 = the legacy default
 stream) and return.  A handle belongs to its device, may be shared by threads,
 streams and captured graphs, and has to outlive the work that was queued with
-it.
+it.  ``close()``, and the last reference to a handle that was not closed, frees
+its device memory: that may wait for the device, and may happen while a graph
+is being captured.  Creating a handle may not.
 """
 
 from __future__ import annotations

@@ -943,6 +943,32 @@ def test_attention_call_refusals():
     assert (out == 5.0).all()
 
 
+@pytest.mark.parametrize("mode", ["global", "thread_local", "relaxed"])
+@pytest.mark.parametrize("other_thread", [False, True])
+def test_handles_freed_inside_a_capture(mode, other_thread):
+    """The last reference to a handle may go while an unrelated graph is captured: the capture goes on."""
+    import threading
+
+    handles = [AttentionPlan(1, 1, 64, [0, 16], dtype="bf16"),
+               Q4Weight.quantize(np.ones((64, 64), np.float32), 32), AxisRope(64, [32])]
+    x = torch.ones(1000, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode=mode):
+        y = x * 2
+        if other_thread:
+            t = threading.Thread(target=handles.clear)
+            t.start()
+            t.join()
+        else:
+            handles.clear()
+        z = y + 1
+    assert not handles
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (z == 3).all()
+
+
 # --------------------------------------------------------------- together --
 
 
