@@ -406,7 +406,7 @@ typedef struct svl_rope_config {
   uint32_t pairs[4];             /* per axis; >= 1 for the first n_axes, 2 * sum <= head_dim */
   uint32_t arrangement;          /* svl_rope_arrangement */
   uint32_t reserved;             /* zero */
-  double theta[4];               /* finite, > 0; theta[0] alone unless SVL_ROPE_SPLIT */
+  double theta[4];               /* finite, >= 1/128; theta[0] alone unless SVL_ROPE_SPLIT */
 } svl_rope_config;
 
 typedef struct svl_rope svl_rope;
@@ -418,8 +418,9 @@ void svl_rope_destroy(svl_rope* rope);
 
 /* Rotates n_tokens rows of q_heads query heads and k_heads key heads (either
  * may be 0) of `dtype` (svl_dtype).  d_positions: n_axes x n_tokens, one axis
- * after another, any int32 values; angles are exact to 2^-32 of a turn however
- * far the position, and products are rounded once to the type.  An output may
+ * after another, any int32 values; however far the position, the angle that sine
+ * and cosine are taken of is within 2^-25 of a turn (2^-26 by its rounding to
+ * FP32), and products are rounded once to the type.  An output may
  * be its own input (same pointer and ld: in place).  Element alignment
  * suffices (4 bytes for the positions; else SVL_USAGE); 16-byte aligned rows with an even head are faster.  heads *
  * head_dim <= ld < 2^36, n_tokens < 2^31 (else SVL_USAGE). */

@@ -5,9 +5,12 @@
 // position * f.  The angle in turns, position * f / 2 pi, is needed modulo 1
 // only, so f / 2 pi is kept as a 64-bit binary fraction of a turn and the
 // product with an integer position wraps in 64-bit arithmetic: the reduction
-// is exact for every int32 position (the fraction's own rounding, 2^-65 of a
-// turn a position, reaches 2^-34 of a turn at 2^31), and FP32 sees an angle in
-// [-1/2, 1/2) turns.
+// is exact for the stored fraction at every int32 position.  The fraction is cut
+// at 2^-64 of a turn, which reaches 2^-33 at 2^31; f / 2 pi itself is computed
+// with 64 significant bits, so where f exceeds a turn (bases below 1) its error
+// is 2^-63 f / 2 pi a position: under 2^-27 of a turn at 2^31 for kLeastTheta,
+// whose largest frequency is 20.4 turns.  sine and cosine see the phase cut at
+// 2^-32 of a turn and rounded to FP32 in [-1/2, 1/2] turns, at most 2^-26 off.
 #include <cmath>
 
 #include "ops_common.cuh"
@@ -18,6 +21,7 @@ namespace svl {
 namespace {
 
 constexpr int kMaxPairs = SVL_ROPE_MAX_HEAD_DIM / 2;
+constexpr double kLeastTheta = 1.0 / 128;
 
 // Passed by value: the tables travel in the launch's own parameters, so the
 // handle owns no device memory and a captured launch keeps its copy.
@@ -193,8 +197,8 @@ int svl_rope_create(const svl_rope_config* config, svl_rope** out, char* err, si
   for (uint32_t a = 0; a < c.n_axes; ++a) {
     if (!c.pairs[a]) return refuse(SVL_USAGE, "every axis needs a pair", err, err_len);
     n += c.pairs[a];
-    if ((a == 0 || c.arrangement == SVL_ROPE_SPLIT) && !(std::isfinite(c.theta[a]) && c.theta[a] > 0))
-      return refuse(SVL_USAGE, "theta must be finite and positive", err, err_len);
+    if ((a == 0 || c.arrangement == SVL_ROPE_SPLIT) && !(std::isfinite(c.theta[a]) && c.theta[a] >= svl::kLeastTheta))
+      return refuse(SVL_USAGE, "theta must be finite and at least 1/128", err, err_len);
   }
   if (2 * n > c.head_dim) return refuse(SVL_USAGE, "the axes' pairs do not fit the head", err, err_len);
   return svl::guarded(err, err_len, [&]() -> int {

@@ -105,7 +105,8 @@ class AxisRope(_Handle):
     arrangement "split": each axis owns its own ``2 * pairs[a]`` dimensions,
     rotate-half inside them, base ``theta[a]``.  "sections" / "interleaved": one
     rotate-half over all pairs with base ``theta[0]``; the axes own runs of
-    pairs, or take them in turn.  Dimensions behind the pairs are copied."""
+    pairs, or take them in turn.  Dimensions behind the pairs are copied.  Bases
+    are at least 1/128."""
 
     _destroy = "svl_rope_destroy"
 

@@ -133,6 +133,35 @@ def test_rope_small_base():
     run_rope("f32", 31, 2, 1, 64, [16, 16], "split", theta=[0.5, 0.01])
 
 
+@pytest.mark.parametrize("theta", [1.0 / 128, 0.01, 0.5, 1.0, 3.0])
+@pytest.mark.parametrize("far", [0, 1 << 20, 2147483000, -2147483648])
+def test_rope_small_bases_far_out(theta, far):
+    """Frequencies of up to 20 turns a position, against angles of 60 digits."""
+    from decimal import Decimal, getcontext
+
+    getcontext().prec = 60
+    turn = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582097494")
+    n, tokens = 16, 40
+    pos = torch.arange(tokens, dtype=torch.int64) + far
+    x = torch.randn(tokens, 2 * n, device="cuda", generator=gen(2))
+    y = torch.empty_like(x)
+    p32 = pos.to(torch.int32).cuda()
+    AxisRope(2 * n, [n], theta).apply_device("f32", p32.data_ptr(), tokens, x.data_ptr(), 2 * n, 1, y.data_ptr(), 2 * n,
+                                             stream=stream())
+    torch.cuda.synchronize()
+    base = Decimal(theta).ln()
+    f = [(-base * i / n).exp() for i in range(n)]
+    angle = np.array([[float((int(p) * w) % turn) for w in f] for p in pos])
+    c, s = np.cos(angle), np.sin(angle)
+    xs, got = x.cpu().double().numpy(), y.cpu().double().numpy()
+    a, b = xs[:, :n], xs[:, n:]
+    size = np.abs(a) + np.abs(b)
+    # the angle within 2^-25 of a turn (6.3 2^-25 rad), sine and cosine within 2 units, two products and a sum rounded
+    tol = size * (6.3 * 2.0 ** -25 + 4 * 2.0 ** -24) + least_half_step("f32")
+    assert (np.abs(got[:, :n] - (a * c - b * s)) <= tol).all()
+    assert (np.abs(got[:, n:] - (b * c + a * s)) <= tol).all()
+
+
 # ----------------------------------------------------------------- linear --
 
 

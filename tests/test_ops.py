@@ -37,6 +37,16 @@ def test_rope_configuration_refusals(kwargs):
         AxisRope(**kwargs)
 
 
+@pytest.mark.parametrize("theta", [1e-3, 1.0 / 129, 5e-324])
+def test_rope_refuses_bases_whose_angles_are_lost(theta):
+    """Frequencies of many turns a position leave too few bits of the angle at far positions; 1/128 is the least base."""
+    with pytest.raises(errors.UsageError):
+        AxisRope(64, [32], theta)
+    with pytest.raises(errors.UsageError):
+        AxisRope(64, [16, 16], [1e4, theta])
+    AxisRope(64, [32], 1.0 / 128).close()
+
+
 def test_rope_c_configuration_refusals():
     lib = load_library()
     for change in (dict(arrangement=3), dict(reserved=1), dict(n_axes=0), dict(n_axes=5)):
