@@ -224,6 +224,34 @@ def test_linear_odd_depth(dtype, k):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 2, 5, 11, 17, 33, 70, 130])
+@pytest.mark.parametrize("k,group", [(96, 32), (160, 32), (1056, 32), (2080, 32), (192, 64), (1088, 64), (2112, 64)])
+def test_linear_last_span_in_part(dtype, rows, k, group):
+    """Depths that end inside a span of 128 columns, in every kernel and with the span run of every rank of a cluster."""
+    run_linear(dtype, rows, 77, k, group, True)
+    run_linear(dtype, rows, 300, k, group, False, scale_dtype="f16")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_linear_padding_behind_a_row_is_not_read_into_it(dtype, rows):
+    """Columns of x behind k, inside the last span or not, may hold anything."""
+    for k, group in ((96, 32), (160, 32), (2112, 64)):
+        g, t, n, ld = gen(k), TYPES[dtype], 50, k + 64
+        codes = torch.randint(0, 256, (n, k // 2), device="cuda", generator=g, dtype=torch.uint8)
+        scales = torch.ones(n, k // group, device="cuda", dtype=torch.bfloat16)
+        x = torch.randn(rows, ld, device="cuda", generator=g).to(t)
+        w = Q4Weight.from_codes(codes.data_ptr(), scales.data_ptr(), n, k, group)
+        ys = []
+        for fill in (0.0, float("nan"), float("inf")):
+            x[:, k:] = fill
+            ys.append(torch.empty(rows, n, device="cuda", dtype=t))
+            w.linear_device(dtype, x.data_ptr(), ld, rows, ys[-1].data_ptr(), n, stream=stream())
+        torch.cuda.synchronize()
+        assert torch.isfinite(ys[0].float()).all() and torch.equal(ys[0], ys[1]) and torch.equal(ys[0], ys[2])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("pad,offset", [(8, 0), (3, 0), (0, 1), (5, 3)])
 def test_linear_strides_and_alignment(dtype, pad, offset):
     run_linear(dtype, 6, 50, 192, 64, False, pad=pad, offset=offset, host=True)
