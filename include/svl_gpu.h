@@ -525,7 +525,7 @@ int svl_q4_read(const svl_q4* weight, uint32_t* n, uint32_t* k, uint32_t* group,
 /* y = x W^T: `rows` rows of x (k values each, row stride ld_x) into y (n
  * values, row stride ld_y), both of `dtype`.  Made for few rows (a query's
  * tokens, down to a single one); any count below 2^31 works.  Products and
- * sums are FP32 (an F32 x keeps its 24 bits), y is rounded once.  A row with a
+ * sums are FP32 (an F32 x keeps its 24 bits, but none below 2^-133), y is rounded once.  A row with a
  * NaN or infinite value gets non-finite results; the others do not.  Element
  * alignment suffices.  Strides are below 2^36.  Columns of y behind n are left
  * as they were. */

@@ -10,7 +10,8 @@
 // whole number of at most 4 bits and sign, exact in FP16 and BF16, so a group's
 // sum of products is FP32-exact up to its additions and the scale multiplies it
 // once in FP32.  FP32 rows are cut into three BF16 parts of 8 bits each, which
-// is exact, and the parts are further columns of the product.
+// is exact for values of 2^-110 and more (BF16 ends at 2^-133, and what lies under
+// that is cut off), and the parts are further columns of the product.
 //
 // 8192 x 28672 with groups of 128 and one BF16 row (121 MB): 36 us, 3.4 TB/s.  The
 // integer pipe bounds it: three shifts and four masks a word of eight codes at half

@@ -280,6 +280,25 @@ def test_linear_large_values_f32():
         assert (np.abs(y.cpu().double().numpy() - xs @ full.T) <= (k + 10) * ULP * (np.abs(xs) @ np.abs(full).T)).all()
 
 
+@pytest.mark.parametrize("rows", [1, 3, 14, 40])
+@pytest.mark.parametrize("power", [-100, -109, -116, -124, -132, -140])
+def test_linear_tiny_values_f32(rows, power):
+    """FP32 values keep their 24 bits down to 2^-110; below, what lies under 2^-133 is cut off."""
+    g, k, n = gen(4), 256, 40
+    codes = torch.randint(0, 256, (n, k // 2), device="cuda", generator=g, dtype=torch.uint8)
+    scales = torch.full((n, k // 32), 2.0 ** 60, device="cuda", dtype=torch.bfloat16)
+    x = (torch.rand(rows, k, device="cuda", generator=g) + 1.0).double().mul(2.0 ** power).float()
+    x *= torch.randint(0, 2, x.shape, device="cuda", generator=g) * 2 - 1
+    y = torch.empty(rows, n, device="cuda")
+    w = Q4Weight.from_codes(codes.data_ptr(), scales.data_ptr(), n, k, 32)
+    w.linear_device("f32", x.data_ptr(), k, rows, y.data_ptr(), n, stream=stream())
+    full = dequantised(codes.cpu().numpy(), np.full((n, k // 32), 2.0 ** 60), None, 32)
+    xs = x.cpu().double().numpy()
+    cut = 2.0 ** -133 * np.abs(full).sum(1) if power < -110 else 0.0
+    bound = (k + 10) * ULP * (np.abs(xs) @ np.abs(full).T) + cut
+    assert (np.abs(y.cpu().double().numpy() - xs @ full.T) <= bound).all()
+
+
 def test_q4_read_returns_what_was_given():
     for zeros in (False, True):
         w, codes, scales, z = run_linear("f32", 1, 37, 160, 32, zeros)
