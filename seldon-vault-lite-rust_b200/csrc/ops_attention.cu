@@ -638,6 +638,15 @@ int svl_attention_plan_create(int device, const svl_attention_config* config, co
     p.doc_k = doc_k ? (const int32_t*)(base + at_doc_k) : nullptr;
     p.blocks = (uint32_t)s.block_segments.size() - 1;
     p.n_joins = (uint32_t)s.joins.size();
+    // a minute, and 4 s more for each 2^17 key tiles of the longest block (30 us a
+    // tile): whole tiles alone, as 32 heads over 2^21 tokens have, outlast any fixed limit
+    uint64_t most_tiles = 0;
+    for (uint32_t b = 0; b < p.blocks; ++b) {
+      uint64_t tiles = 0;
+      for (uint32_t i = s.block_segments[b]; i < s.block_segments[b + 1]; ++i) tiles += s.segments[i].list1 - s.segments[i].list0;
+      most_tiles = std::max(most_tiles, tiles);
+    }
+    p.check_waits = 15 + (uint32_t)(most_tiles >> 17);
     p.q_heads = c.q_heads;
     p.kv_heads = c.kv_heads;
     p.group = group;

@@ -51,6 +51,7 @@ struct AttnParams {
   const float* slopes;   // NULL without a distance bias
   uint32_t* err;
   uint32_t blocks, n_joins, slot_rows;
+  uint32_t check_waits;  // a check warp's patience, in waits (4 s)
   uint32_t q_heads, kv_heads, group, head_dim;
   uint64_t total_q, total_k;
   float scale, cap;

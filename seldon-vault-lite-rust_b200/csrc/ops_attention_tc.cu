@@ -382,9 +382,9 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
       // ------------------------------------------------------------ checks --
       const int tid = threadIdx.x - 64;
       for (uint32_t round = 0;; ++round) {
-        // between two checks lies any number of fully seen tiles: the limit is 15 times a wait's
+        // between two checks lies any number of fully seen tiles: the limit goes by the block's tiles
         bool got = false;
-        for (int i = 0; !got && i < 15; ++i) got = mbar_wait(&sm.check_req, round & 1, nullptr);
+        for (uint32_t i = 0; !got && i < p.check_waits; ++i) got = mbar_wait(&sm.check_req, round & 1, nullptr);
         if (!got) {
           atomicOr(p.err, SVL_DEVERR_TIMEOUT);
           break;
