@@ -306,10 +306,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
             const RingPos v = pos, k = ahead(pos, 1, stages);
             wait(&sm.full[v.stage], v.phase);
             if (more) wait(&sm.full[k.stage], k.phase);
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-              if (sees_any(e, t) && !started[t]) ++turn[t];
-            if (some(e)) ask(v, sees_any(e, 0) ? turn[0] : 0, sees_any(e, 1) ? turn[1] : 0);
+            if (some(e)) ask(v, sees_any(e, 0) ? turn[0] + !started[0] : 0, sees_any(e, 1) ? turn[1] + !started[1] : 0);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
               const bool now = sees_any(e, t), then = more && sees_any(e1, t);
@@ -323,6 +320,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
                 if (then) scores(t, t, k, t == 1 || !sees_any(e1, 1));
               }
               __syncwarp();
+              turn[t] += now && !started[t];
               started[t] |= now;
             }
             if (j + 2 == n && ok && elect_one()) mma_commit(&sm.q_empty);
@@ -539,7 +537,9 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
           if (plain) top *= scale2;
           if (capped) {
             small = !__any_sync(0xffffffffu, live && fmaxf(top, -low) > p.cap_limit);
-            top = top == -INFINITY ? top : capped_any(p, top, cap_arg, cap2);  // the cap keeps the order
+            // the cap keeps the order
+            const float by = small ? capped_small(p, top) : capped_any(p, top, cap_arg, cap2);
+            top = top == -INFINITY ? top : by;
           }
         } else
 #pragma unroll 1
