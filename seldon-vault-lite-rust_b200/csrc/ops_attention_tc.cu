@@ -37,6 +37,11 @@ namespace svl {
 namespace {
 
 constexpr int kCols = 64;  // score columns of a softmax thread
+// Behind this size (log2 units) a score and its bias are rounded before the maximum
+// is subtracted.  Below it the subtraction may share a multiply-add with the product
+// and the bias may run along the columns in steps: the maximum and the exponents then
+// differ by up to 16 2^-24 of the size, at most 1, where a weight has to stay below 2^16.
+constexpr float kMild = 1048576.0f;
 // Tensor-memory columns of the weights of keys 16 k ..: each thread's lie over its own scores.
 SVL_DEV uint32_t weights_at(int k) { return k * 16 / kCols * kCols + k * 16 % kCols / 2; }
 
@@ -485,20 +490,21 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
           for (int h = 0; h < 2; ++h)
             if (j0 + 32 * h + lane < (int64_t)s.n_k) docs[h] = __ldg(p.doc_k + s.k0 + j0 + 32 * h + lane);
         }
-        wait(&sm.s_full[buf], (kTiles == 2 ? g : g >> 1) & 1);
-        tc_fence_after();
         const uint32_t s_addr = lane_addr + buf * 128 + half * kCols;
         // Tiles that a row sees whole need nothing but the maximum (and, for the
         // cap, the minimum) here, and their scores are transformed where they are
         // exponentiated.  The distance is linear over columns that the row's own
-        // place does not lie among.  In all other cases the transformed scores go
-        // back to TMEM.
+        // place does not lie among; the bias has to be mild over them.  In all other
+        // cases the transformed scores go back to TMEM.
         const float gap = (float)(mask.place - j0);
-        const bool apart_from = gap >= (float)(kCols - 1) || gap <= 0.0f;
+        const bool apart_from = (gap >= (float)(kCols - 1) || gap <= 0.0f) && fabsf(slope2) * (fabsf(gap) + kCols) <= kMild;
         const bool direct = see == kSeesAll && (plain || (capped != biased && (capped ? mild_cap : __all_sync(0xffffffffu, apart_from))));
         const float rise = gap > 0.0f ? slope2 : -slope2;  // direct bias: -slope |gap - c| = rise (c - gap)
+        wait(&sm.s_full[buf], (kTiles == 2 ? g : g >> 1) & 1);
+        tc_fence_after();
         float top = -INFINITY;
-        bool small = true;  // every score within the cap's polynomial
+        bool small = true;   // every score within the cap's polynomial
+        bool raw = direct;   // the scores in TMEM stay as they are
         if (direct) {
           float low = INFINITY;
 #pragma unroll 1
@@ -540,8 +546,12 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
             // the cap keeps the order
             const float by = small ? capped_small(p, top) : capped_any(p, top, cap_arg, cap2);
             top = top == -INFINITY ? top : by;
+          } else {
+            raw = !__any_sync(0xffffffffu, live && fabsf(top) > kMild);
+            if (!raw) top = -INFINITY;
           }
-        } else
+        }
+        if (!raw)
 #pragma unroll 1
         for (int c0 = 0; c0 < kCols; c0 += 32) {
           uint32_t w[32];
@@ -659,7 +669,7 @@ __global__ void __launch_bounds__(Shape<HDP>::kThreads, 1)
           }
         };
         const uint64_t base2 = two(-base, -base);
-        if (!direct) {
+        if (!raw) {
           weights([&](uint64_t* y, int) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = add_two(y[i], base2);

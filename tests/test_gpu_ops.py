@@ -894,6 +894,58 @@ def test_attention_large_caps_reached(dtype, by, n_q, n_k, hd, of_scores):
     assert ((out.double() - 1).abs() <= tol).all() and torch.isfinite(lse).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n_q,n_k,hd", [(256, 256, 64), (256, 512, 128), (130, 256, 256), (2, 512, 128)])
+@pytest.mark.parametrize("by", [300.0, 3e3, 1.2e4])
+def test_attention_scores_far_above_one(dtype, by, n_q, n_k, hd):
+    """Scores of 1e6 to 1e10, where FP32 steps over whole units: a weighted mean of ones is one, and the log sum is the
+    largest score."""
+    g, t = gen(9), TYPES[dtype]
+    q = (torch.randn(n_q, hd, device="cuda", generator=g) * by).to(t)
+    k = (torch.randn(n_k, hd, device="cuda", generator=g) * by).to(t)
+    v = torch.ones(n_k, hd, device="cuda", dtype=t)
+    out, lse = attend(AttentionPlan(1, 1, hd, [0, n_q], [0, n_k], dtype=dtype, scale=1.0), q, k, v, 1, hd)
+    tol = 2 * half_step(dtype) + 2 * (n_k + 4) * ULP
+    assert ((out.double() - 1).abs() <= tol).all()
+    top, size = (q.double() @ k.double().T).amax(1), (q.double().abs() @ k.double().abs().T).amax(1)
+    # hd products, a scale in log2 units and back; at most n_k scores as large as the largest
+    assert ((lse[:, 0].double() - top).abs() <= (hd + 8) * ULP * size + math.log(n_k)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("slope", [1e3, -1e3, 1e5, -1e5, 1e12, -1e12, 1e20, -1e20])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [2, 300])
+def test_attention_steep_slopes(dtype, slope, hd, rows):
+    """Slopes of any allowed size, keys near and far preferred: the mean of ones is one, the values are the preferred
+    keys', and the log sum is their score and bias."""
+    n_k, t = 900, TYPES[dtype]
+    for docs in (None, [0] * 400 + [1] * 500):
+        q = torch.randn(rows, 2 * hd, device="cuda", generator=gen(1)).to(t)
+        k = torch.randn(n_k, hd, device="cuda", generator=gen(2)).to(t)
+        v = torch.ones(n_k, hd, device="cuda", dtype=t)
+        where = torch.arange(n_k, device="cuda") % 64  # exact in every type
+        v[:, 1] = where.to(t)
+        # with documents the rows are the first one's: every key that they see is far away
+        plan = AttentionPlan(2, 1, hd, [0, rows], [0, n_k], dtype=dtype, slopes=[slope, slope / 4],
+                             doc_q=None if docs is None else [0] * rows, doc_k=docs)
+        out, lse = attend(plan, q, k, v, 2, hd)
+        out = out.view(rows, 2, hd)
+        tol = 2 * half_step(dtype) + 2 * (n_k + 4) * ULP
+        assert ((out[..., 2:].double() - 1).abs() <= tol).all()
+        p = torch.arange(n_k - rows, n_k, device="cuda")
+        seen = 400 if docs else n_k
+        at = p.clamp(max=seen - 1) if slope > 0 else torch.zeros_like(p)  # nearest or farthest, unless two are as far
+        for h, s in enumerate((slope, slope / 4)):
+            gap = (p - at).abs().double()
+            score = (q.view(rows, 2, hd)[:, h].double() * k[at].double()).sum(1) * hd ** -0.5 - s * gap
+            far = (gap > 0) | (slope > 0)
+            err = (lse[:, h].double() - score).abs()
+            assert (err[far] <= 1e-3 + 8 * ULP * abs(s) * (gap[far] + 64)).all()
+            if abs(s) * (gap.max() + 64) * 16 * ULP < 1:  # FP32 tells neighbours apart: one key has all the weight
+                assert (out[:, h, 1].double() - where[at].double()).abs().max() <= 64 * tol
+
+
 FIRST_CALLS = """
 import sys
 sys.path.insert(0, {pkg!r})
