@@ -576,6 +576,24 @@ def test_attention_heads(dtype, hq, hk, hd):
     run_attention(dtype, hq, hk, hd, [(1, 1), (130, 130), (45, 45)])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [8, 16, 24, 40, 48, 56, 88, 104, 112, 120, 136, 160, 168, 200, 216, 240, 248])
+@pytest.mark.parametrize("kwargs", [dict(cap=4.0, causal=True), dict(slopes=True), dict(docs=shuffled, prefix=[3, 40])],
+                         ids=lambda d: ",".join(d))
+def test_attention_every_head_size(dtype, hd, kwargs):
+    """Heads that end inside a slab of 64 columns or a step of 16, for the tiles and for few rows."""
+    run_attention(dtype, 3, 1, hd, [(130, 130), (301, 301)], **kwargs)
+    run_attention(dtype, 3, 1, hd, [(2, 400), (1, 129)], **kwargs)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("group", [3, 7, 12, 33, 60, 65, 100, 127, 128])
+@pytest.mark.parametrize("hd", [64, 136])
+def test_attention_every_group(dtype, group, hd):
+    """Row tiles of whole queries that leave rows of the tile empty."""
+    run_attention(dtype, group, 1, hd, [(9, 9), (70, 200)], cap=4.0, causal=True)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("kwargs", [
     {}, dict(causal=True), dict(window=0), dict(window=40), dict(causal=True, window=130), dict(cap=5.0),
