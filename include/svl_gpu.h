@@ -372,8 +372,8 @@ int svl_search_noalloc(const float* d_rows, const uint64_t* d_chunk_ids, uint64_
  * referring to the handle, which has to outlive the graph, and a queued one
  * has to be over before its handle is destroyed.  Destroying a handle frees its
  * memory at once and may wait for the device; it may happen while a capture
- * is open, on any thread.  Creating one allocates, copies and waits, and is not
- * for an open capture.  A handle is never changed by a call, so threads,
+ * is open, on any thread.  Creating or reading one allocates, copies and waits,
+ * and checking a plan waits: not for an open capture.  A handle is never changed by a call, so threads,
  * streams and graphs may share it; outputs and workspaces are the caller's
  * and must not be shared by calls that may overlap.  Outputs must not overlap
  * inputs except where stated.  NULL pointers are accepted where nothing is
@@ -442,8 +442,9 @@ int svl_rope_apply_device(const svl_rope* rope, int device, uint32_t dtype, cons
  * A row that sees no key gets out = 0 and lse = -inf.  A masked key's values
  * never reach a row, be they NaN or infinite; rows of other sequences and
  * rows behind the last one are neither read into a result nor written.
- * Scores, softmax statistics and sums are FP32 (FP16 / BF16: the weights of
- * the visible keys are rounded to the type before they multiply v). */
+ * Scores, softmax statistics and sums are FP32 (a capped score is off by up to
+ * 2^-20 of the cap where it comes near it; FP16 / BF16: the weights of the
+ * visible keys are rounded to the type before they multiply v). */
 typedef struct svl_attention_config {
   uint32_t dtype;                /* svl_dtype of q, k, v and out */
   uint32_t q_heads;              /* a multiple of kv_heads; q_heads / kv_heads <= 65535 */

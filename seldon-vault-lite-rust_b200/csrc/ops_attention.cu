@@ -658,13 +658,17 @@ int svl_attention_plan_create(int device, const svl_attention_config* config, co
     if (c.cap > 0) {
       const double k = (double)c.scale / c.cap;
       double power = (double)c.cap * 1.4426950408889634 * k;
-      // a coefficient that FP32 cannot hold leaves every score to the general form
+      // A coefficient too large for FP32 leaves every score to the general form.  One
+      // too small is left out, and the polynomial ends where it would be 2^-25 of it.
       bool held = true;
+      double limit = svl::kTanhLimit;
       for (int i = 0; i < svl::kCapTerms; ++i, power *= k * k) {
+        const bool small = std::fabs(power * svl::kTanhOdd[i]) < 1e-37;
+        if (small) limit = std::min(limit, svl::kTanhWithout[i]);
         held &= std::fabs(power) < 1e37;
-        p.cap_odd[i] = held ? (float)(power * svl::kTanhOdd[i]) : 0.0f;
+        p.cap_odd[i] = held && !small ? (float)(power * svl::kTanhOdd[i]) : 0.0f;
       }
-      p.cap_limit = held ? (float)std::min(svl::kTanhLimit / k, 3.0e38) : -1.0f;
+      p.cap_limit = held ? (float)std::min(limit / k, 1.8e19) : -1.0f;  // whose square is finite
     }
     p.causal = (int32_t)c.causal;
     p.window = c.window;

@@ -18,11 +18,14 @@ constexpr float kBehind = 8.0f;  // a maximum follows once it is 2^8 behind (log
 // FP32's half step): multiply-adds on the FMA pipe, with the cap and scale in the
 // coefficients.  The general form costs two of the 16 special functions a cycle
 // that the softmax itself needs, and its error is of the cap's size.  A score takes
-// it behind cap_limit = 0.35 cap / scale, and by its own size alone: what else the
+// it behind cap_limit (0.35 cap / scale), and by its own size alone: what else the
 // tile holds (masked keys, other sequences, rows behind the tile) decides only
 // whether the warp computes the general form at all.
 constexpr double kTanhOdd[kCapTerms] = {0.9999999659298247, -0.3333243239119307, 0.1329601580300818, -0.04897000350211587};
 constexpr double kTanhLimit = 0.35;
+// where term i of it is 2^-25 of the whole: the limit without that term (its
+// coefficient shrinks with the cap: caps above 2e5 at a scale of 1/8 lose the last one)
+constexpr double kTanhWithout[kCapTerms] = {0.0, 2.9e-4, 0.0217, 0.092};
 SVL_DEV float cap_odd(const AttnParams& p, float s) {
   const float z = __fmul_rn(s, s);
   return fmaf(z, fmaf(z, fmaf(z, p.cap_odd[3], p.cap_odd[2]), p.cap_odd[1]), p.cap_odd[0]);

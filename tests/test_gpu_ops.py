@@ -964,6 +964,28 @@ def test_attention_steep_slopes(dtype, slope, hd, rows):
                 assert (out[:, h, 1].double() - where[at].double()).abs().max() <= 64 * tol
 
 
+@pytest.mark.parametrize("dtype,by", [("f32", 1.0), ("f32", 3e4), ("f32", 3e8), ("bf16", 1.0), ("bf16", 60.0), ("bf16", 3e4),
+                                      ("bf16", 3e8), ("f16", 1.0), ("f16", 60.0), ("f16", 1e3)])
+@pytest.mark.parametrize("n_q,n_k", [(256, 256), (2, 512)])
+@pytest.mark.parametrize("of_cap", [1e-4, 1e-3, 0.01, 0.05, 0.2, 0.3, 0.34, 1.0])
+def test_attention_scores_near_a_large_cap(dtype, by, n_q, n_k, of_cap):
+    """Caps of any size whose scores reach a given part of them: the log sum, which is the largest score's, is off by units
+    of the cap at most."""
+    g, t, hd = gen(9), TYPES[dtype], 64
+    q = (torch.randn(n_q, hd, device="cuda", generator=g) * by).to(t)
+    k = (torch.randn(n_k, hd, device="cuda", generator=g) * by).to(t)
+    s = q.double() @ k.double().T
+    cap = float(np.float32(s.abs().max().item() / of_cap))
+    out, lse = attend(AttentionPlan(1, 1, hd, [0, n_q], [0, n_k], dtype=dtype, scale=1.0, cap=cap), q, k, torch.ones_like(k), 1, hd)
+    want = torch.logsumexp(cap * torch.tanh(s / cap), 1)
+    size = (q.double().abs() @ k.double().abs().T).amax(1)
+    # as in attention_reference: hd products and a scale; 8 units of the cap for tanh; 4 of the cap and of the result
+    tol = (hd + 4) * ULP * size + 12 * ULP * cap + (n_k + 16) * ULP + 5 * ULP * want.abs()
+    err = (lse[:, 0].double() - want).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+    assert ((out.double() - 1).abs() <= 2 * half_step(dtype) + 2 * (n_k + 4) * ULP).all()
+
+
 FIRST_CALLS = """
 import sys
 sys.path.insert(0, {pkg!r})
