@@ -10,8 +10,8 @@
 // K and V come by TMA through a ring of 16 KB slabs that a thread of a third
 // warpgroup keeps full across tiles and segments; its registers go to the teams.
 // One row of 32 query and 8 key heads of 128 over 8 caches of 13135-64537 keys
-// (1.25 GB): 250 us, 5.0 TB/s; bound by the instructions of eight warps (0.31 a
-// cycle and scheduler), then by memory.
+// (1.25 GB): 250-258 us, 4.8-5.0 TB/s; bound by the chains of two warps a scheduler,
+// which issue in 27% of the cycles, then by memory.
 #include "ops_attention_mma.cuh"
 
 namespace svl {

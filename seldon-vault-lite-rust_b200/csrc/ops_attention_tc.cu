@@ -26,11 +26,12 @@
 // and the epilogue adds them back to the rows that see them.
 //
 // What bounds it: the round from a row tile's scores through its softmax and back
-// to the products.  On that case (440 us, 786 TFLOP/s counted over visible pairs)
-// the products alone, with the softmax only handing over, take 307 us; S reads
-// both operands from shared memory, 8 KB a 64-cycle step, which is all its
-// bandwidth.  Leaving out the cap's polynomial saves 63 us, the maximum 45, the
-// exponentials 26.
+// to the products.  On that case (437-474 us from box to box, 730-790 TFLOP/s
+// counted over visible pairs) the products alone, with the softmax only handing
+// over, take 307 us; S reads both operands from shared memory, 8 KB a 64-cycle step,
+// which is all its bandwidth.  Of 440 us, leaving out the cap's polynomial saves 63,
+// the maximum 45, the exponentials 26.  On a shorter such batch the tensor pipe is
+// active 36% of the cycles, the special functions 37%, and a scheduler issues in 54%.
 #include "ops_attention_mma.cuh"
 
 namespace svl {

@@ -13,9 +13,9 @@
 // is exact for values of 2^-110 and more (BF16 ends at 2^-133, and what lies under
 // that is cut off), and the parts are further columns of the product.
 //
-// 8192 x 28672 with groups of 128 and one BF16 row (121 MB): 36 us, 3.4 TB/s.  The
-// integer pipe bounds it: three shifts and four masks a word of eight codes at half
-// an instruction a cycle and scheduler, 71% busy while the kernel runs.
+// 8192 x 28672 with groups of 128 and one BF16 row (121 MB): 36-38 us, 3.2-3.4 TB/s.
+// The integer pipe bounds it: three shifts and four masks a word of eight codes at half
+// an instruction a cycle and scheduler, 70-71% busy while the kernel runs.
 #include <algorithm>
 #include <cmath>
 #include <cstddef>

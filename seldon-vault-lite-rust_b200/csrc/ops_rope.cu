@@ -63,7 +63,7 @@ struct alignas(sizeof(T) * V) Pack {
 // order, V pairs a thread.  Bound by reading and writing the rows once.  (A
 // thread that keeps the angles of one token and turns them in several heads saves
 // the shared memory, but spreads the block's accesses over that many rows at a
-// time: 173 against 130 us for 65536 BF16 rows of 20 heads of 128, 5.2 TB/s.)  The last vectors
+// time: 173 against 130 us for 65536 BF16 rows of 20 heads of 128, 5.1-5.2 TB/s.)  The last vectors
 // of a head copy the dimensions behind the pairs.
 template <typename T, int V>
 __global__ void __launch_bounds__(512)
