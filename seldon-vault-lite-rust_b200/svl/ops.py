@@ -163,6 +163,8 @@ class AttentionPlan(_Handle):
         if window is not None:
             window = _count(window, "window", (1 << 31) - 1)
         head_dim = _count(head_dim, "head_dim")
+        if cap and not ctypes.c_float(cap).value:
+            raise errors.UsageError("cap is neither 0 nor in 1e-30..=1e30")
         c = SvlAttentionConfig(dtype=_dtype(dtype), q_heads=_count(q_heads, "q_heads"),
                                kv_heads=_count(kv_heads, "kv_heads"), head_dim=head_dim,
                                scale=float(max(head_dim, 1) ** -0.5 if scale is None else scale), cap=float(cap),

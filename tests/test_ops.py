@@ -120,6 +120,13 @@ def test_attention_plan_limits(change):
         AttentionPlan(**{**PLAN, **change})
 
 
+@pytest.mark.parametrize("cap", [1e-46, 1e-300, -1e-46])
+def test_attention_refuses_caps_that_round_to_none(cap):
+    """A cap too small for the C float would arrive as 0, which is no cap."""
+    with pytest.raises(errors.UsageError):
+        AttentionPlan(**PLAN, cap=cap)
+
+
 def test_attention_c_configuration_refusals():
     lib = load_library()
     cu = np.array([0, 4], np.uint64)
