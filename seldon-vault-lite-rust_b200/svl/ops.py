@@ -51,7 +51,10 @@ def _dtype(name: str) -> int:
 
 def _count(value, what: str, most: int = (1 << 32) - 1) -> int:
     """A whole number that fits its C argument (ctypes would cut it)."""
-    n = int(value)
+    try:
+        n = int(value)
+    except (ValueError, OverflowError):  # NaN, infinities
+        n = -1
     if n != value or not 0 <= n <= most:
         raise errors.UsageError(f"{what} must be a whole number in 0..={most}")
     return n

@@ -127,6 +127,16 @@ def test_attention_refuses_caps_that_round_to_none(cap):
         AttentionPlan(**PLAN, cap=cap)
 
 
+@pytest.mark.parametrize("build", [
+    lambda x: AxisRope(64, [x]), lambda x: AxisRope(x, [8]), lambda x: AttentionPlan(**{**PLAN, "q_heads": x}),
+    lambda x: AttentionPlan(**PLAN, window=x), lambda x: Q4Weight.from_codes(FAKE, FAKE, x, 64, 32),
+])
+@pytest.mark.parametrize("x", [float("nan"), float("inf"), 2.5])
+def test_counts_that_are_no_whole_numbers(build, x):
+    with pytest.raises(errors.UsageError):
+        build(x)
+
+
 def test_attention_c_configuration_refusals():
     lib = load_library()
     cu = np.array([0, 4], np.uint64)
