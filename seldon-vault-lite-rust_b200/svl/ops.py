@@ -138,6 +138,8 @@ class AxisRope(_Handle):
                      device: int = 0, stream: int = 0) -> None:
         """Rotates ``n_tokens`` rows of ``q_heads`` and ``k_heads`` heads; ``positions``
         holds ``n_axes`` x ``n_tokens`` int32.  In place where an output is its input."""
+        if (q_heads | k_heads) >> 32:  # ctypes would cut them
+            raise errors.UsageError("more than 65535 heads")
         eb = _thread.err
         rc = self._lib.svl_rope_apply_device(self._h, device, _dtype(dtype), positions, n_tokens, q, ld_q, q_heads,
                                              q_out, ld_q_out, k, ld_k, k_heads, k_out, ld_k_out, stream or None,

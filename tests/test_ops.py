@@ -89,6 +89,14 @@ def test_rope_refuses_misaligned_positions(offset):
         AxisRope(64, [32]).apply_device(**call)
 
 
+@pytest.mark.parametrize("change", [dict(q_heads=(1 << 32) + 2), dict(k_heads=(1 << 32) + 1), dict(q_heads=-2)])
+def test_rope_refuses_head_counts_that_would_be_cut(change):
+    call = dict(dtype="f32", positions=FAKE, n_tokens=0, q=FAKE, ld_q=128, q_heads=2, q_out=2 * FAKE, ld_q_out=128,
+                k=FAKE, ld_k=64, k_heads=1, k_out=2 * FAKE, ld_k_out=64)
+    with pytest.raises(errors.UsageError):
+        AxisRope(64, [32]).apply_device(**{**call, **change})
+
+
 def test_rope_of_nothing_needs_no_device():
     AxisRope(64, [32]).apply_device("f32", 0, 0, 0, 0, 2, 0, 0)
     AxisRope(64, [32]).apply_device("f32", 0, 9, 0, 0, 0, 0, 0)
