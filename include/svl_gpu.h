@@ -373,9 +373,9 @@ int svl_search_noalloc(const float* d_rows, const uint64_t* d_chunk_ids, uint64_
  * has to be over before its handle is destroyed.  Destroying a handle frees its
  * memory at once and may wait for the device; it may happen while a capture
  * is open, on any thread.  Creating or reading one allocates, copies and waits,
- * and checking a plan waits: not for an open capture.  A handle is never changed by a call, so threads,
- * streams and graphs may share it; outputs and workspaces are the caller's
- * and must not be shared by calls that may overlap.  Outputs must not overlap
+ * and checking a plan waits: not for an open capture.  A handle is never
+ * changed by a call, so threads, streams and graphs may share it; outputs and
+ * workspaces are the caller's and must not be shared by calls that may overlap.  Outputs must not overlap
  * inputs except where stated.  NULL pointers are accepted where nothing is
  * read or written through them. */
 

@@ -42,6 +42,7 @@ constexpr int kCols = 64;  // score columns of a softmax thread
 // is subtracted.  Below it the subtraction may share a multiply-add with the product
 // and the bias may run along the columns in steps: the maximum and the exponents then
 // differ by up to 16 2^-24 of the size, at most 1, where a weight has to stay below 2^16.
+// The rows of a warp (all of one sequence) share the choice.
 constexpr float kMild = 1048576.0f;
 // Tensor-memory columns of the weights of keys 16 k ..: each thread's lie over its own scores.
 SVL_DEV uint32_t weights_at(int k) { return k * 16 / kCols * kCols + k * 16 % kCols / 2; }
