@@ -109,20 +109,34 @@ __global__ void __launch_bounds__(kGenThreads, 2) attention_general_kernel(const
         }
         if (tid < kGenKeys) s_doc[tid] = p.doc_k && j0 + tid < s.n_k ? p.doc_k[s.k0 + j0 + tid] : 0;
         __syncthreads();
+        // four sums of every fourth dimension over 64 dimensions at a time: a rounding
+        // is of a sum of 16 products, not of the whole head
         float dot[M][M] = {};
+        for (uint32_t d0 = 0; d0 < hd; d0 += 64) {
+          float4 part[M][M] = {};
+          const uint32_t d1 = min(d0 + 64, hd);
 #pragma unroll 4
-        for (uint32_t d = 0; d < hd; d += 4) {  // the strides' padding is zero
-          float4 a[M], b[M];
+          for (uint32_t d = d0; d < d1; d += 4) {  // the strides' padding is zero
+            float4 a[M], b[M];
 #pragma unroll
-          for (int u = 0; u < M; ++u) {
-            a[u] = *(const float4*)(sq + (M * ty + u) * stride + d);
-            b[u] = *(const float4*)(sk + (tx + kSpan * u) * stride + d);
+            for (int u = 0; u < M; ++u) {
+              a[u] = *(const float4*)(sq + (M * ty + u) * stride + d);
+              b[u] = *(const float4*)(sk + (tx + kSpan * u) * stride + d);
+            }
+#pragma unroll
+            for (int u = 0; u < M; ++u)
+#pragma unroll
+              for (int w = 0; w < M; ++w) {
+                part[u][w].x = fmaf(a[u].x, b[w].x, part[u][w].x);
+                part[u][w].y = fmaf(a[u].y, b[w].y, part[u][w].y);
+                part[u][w].z = fmaf(a[u].z, b[w].z, part[u][w].z);
+                part[u][w].w = fmaf(a[u].w, b[w].w, part[u][w].w);
+              }
           }
 #pragma unroll
           for (int u = 0; u < M; ++u)
 #pragma unroll
-            for (int w = 0; w < M; ++w)
-              dot[u][w] = fmaf(a[u].x, b[w].x, fmaf(a[u].y, b[w].y, fmaf(a[u].z, b[w].z, fmaf(a[u].w, b[w].w, dot[u][w]))));
+            for (int w = 0; w < M; ++w) dot[u][w] += (part[u][w].x + part[u][w].y) + (part[u][w].z + part[u][w].w);
         }
 #pragma unroll
         for (int u = 0; u < M; ++u)

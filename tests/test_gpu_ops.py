@@ -986,6 +986,21 @@ def test_attention_scores_near_a_large_cap(dtype, by, n_q, n_k, of_cap):
     assert ((out.double() - 1).abs() <= 2 * half_step(dtype) + 2 * (n_k + 4) * ULP).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 200, 256, 512])
+@pytest.mark.parametrize("n_q", [1, 3, 200])
+def test_attention_f32_scores_are_summed_in_parts(hd, n_q):
+    """The log sum over one key is its score.  Values just above 1, whose excess a running sum near the head's size would
+    lose in every step: sums of 16 products, two additions, one for each 64 dimensions and the scale's rounding."""
+    value = 1.0 + 0.49 * 2.0 ** -24 * hd
+    q = torch.full((n_q, hd), value, device="cuda")
+    k = torch.ones(n_q, hd, device="cuda")
+    cu = list(range(n_q + 1))
+    out, lse = attend(AttentionPlan(1, 1, hd, cu, cu, dtype="f32", scale=1.0), q, k, k, 1, hd)
+    want = hd * float(np.float32(value))
+    assert ((lse.double() - want).abs() <= (16 + 2 + hd / 64 + 1) * 2.0 ** -24 * want).all()
+    assert (out == 1.0).all()
+
+
 FIRST_CALLS = """
 import sys
 sys.path.insert(0, {pkg!r})
